@@ -607,6 +607,7 @@ struct DecodeParams {
   const int* kv_lens;
   int max_blocks, block_size, nq, nkv, splits;
   int num_blocks;     // blocks in the cache (bounds checks)
+  int window, sinks;  // sliding-window kernel only
   float scale;
   bf16* o;            // [B, nq, D]
   float* part_o;      // [B, nq, splits, D]  (splits > 1)
@@ -620,8 +621,10 @@ struct DecodeParams {
 // so a tile costs one barrier.  The warp-merge area aliases the ring.
 constexpr int DEC_STAGES = 2;   // default ring depth (x 3 resident CTAs per SM)
 
+// WIN: keys before `lo` that are no sinks are not loaded either (zeros: a NaN there must not reach the row)
+template <bool WIN = false>
 __device__ __forceinline__ void dec_load_tile(bf16* sm, const bf16* cache, const int* bt_row, int block_size,
-                                              int nkv, int kvh, int key0, int k_end, int b, int num_blocks) {
+                                              int nkv, int kvh, int key0, int k_end, int b, int num_blocks, int lo = 0, int sinks = 0) {
   // BN rows x 16 chunks of 16 B; 128 threads -> 8 chunks each
   if (block_size % BN == 0) {
     // tiles start on multiples of BN, so the whole tile sits in one cache
@@ -633,7 +636,7 @@ __device__ __forceinline__ void dec_load_tile(bf16* sm, const bf16* cache, const
     for (int i = 0; i < BN * 16 / NTHREADS; ++i) {
       const int idx = threadIdx.x + i * NTHREADS;
       const int r = idx >> 4, c = idx & 15;
-      const bool ok = key0 + r < k_end && blk >= 0;
+      const bool ok = key0 + r < k_end && blk >= 0 && (!WIN || key0 + r >= lo || key0 + r < sinks);
       cp_async16(sm + swz(r, c * 8), ok ? base + r * D + c * 8 : cache, ok);
     }
     return;
@@ -643,7 +646,7 @@ __device__ __forceinline__ void dec_load_tile(bf16* sm, const bf16* cache, const
     const int idx = threadIdx.x + i * NTHREADS;
     const int r = idx >> 4, c = idx & 15;
     const int key = key0 + r;
-    bool ok = key < k_end;
+    bool ok = key < k_end && (!WIN || key >= lo || key < sinks);
     const bf16* src = cache;
     if (ok) {
       const int blk = bt_row[key / block_size];
@@ -654,7 +657,9 @@ __device__ __forceinline__ void dec_load_tile(bf16* sm, const bf16* cache, const
   }
 }
 
-template <int STAGES>
+// WIN: sliding window with sinks.  The visible 64-key tiles are the sinks' tiles
+// [0, ns) and then the window's, w0 ..; they are what the splits share out.
+template <int STAGES, bool WIN>
 __device__ __forceinline__ void decode_body(const DecodeParams& p) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
   bf16* sQ = reinterpret_cast<bf16*>(smem_raw);  // [16][D]
@@ -665,10 +670,19 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
 
   const int b = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
   const int grp = p.nq / p.nkv;
-  const int kv_len = chk::clamp_to(p.kv_lens[b], p.max_blocks * p.block_size, 63, b);
+  int kv_len = chk::clamp_to(p.kv_lens[b], p.max_blocks * p.block_size, 63, b);
+  if (WIN) kv_len = max(0, min(kv_len, p.max_blocks * p.block_size));
+  const int lo = WIN ? max(0, kv_len - p.window) : 0;  // first key of the window
+  const int w0 = lo / BN, ns = WIN ? min((min(p.sinks, lo) + BN - 1) / BN, w0) : 0;
   const int per = (((kv_len + p.splits - 1) / p.splits) + BN - 1) / BN * BN;
   const int k_begin = split * per;
-  const int k_end = min(kv_len, k_begin + per);
+  const int k_end = WIN ? kv_len : min(kv_len, k_begin + per);
+  const int all = ns + (kv_len + BN - 1) / BN - w0, share = (all + p.splits - 1) / p.splits;  // WIN: tiles
+  auto key_of = [&](int t) {
+    if (!WIN) return k_begin + t * BN;
+    const int v = split * share + t;
+    return (v < ns ? v : v - ns + w0) * BN;
+  };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int* bt_row = p.block_table + (int64_t)b * p.max_blocks;
 
@@ -683,14 +697,14 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
   }
   cp_async_commit();
 
-  const int n_tiles = k_end > k_begin ? (k_end - k_begin + BN - 1) / BN : 0;
+  const int n_tiles = WIN ? max(0, min(share, all - split * share)) : k_end > k_begin ? (k_end - k_begin + BN - 1) / BN : 0;
 #pragma unroll
   for (int st = 0; st < STAGES - 1; ++st) {
     if (st < n_tiles) {
-      dec_load_tile(sK + st * BN * D, p.kc, bt_row, p.block_size, p.nkv, kvh, k_begin + st * BN, k_end, b,
-                    p.num_blocks);
-      dec_load_tile(sV + st * BN * D, p.vc, bt_row, p.block_size, p.nkv, kvh, k_begin + st * BN, k_end, b,
-                    p.num_blocks);
+      dec_load_tile<WIN>(sK + st * BN * D, p.kc, bt_row, p.block_size, p.nkv, kvh, key_of(st), k_end, b,
+                    p.num_blocks, lo, p.sinks);
+      dec_load_tile<WIN>(sV + st * BN * D, p.vc, bt_row, p.block_size, p.nkv, kvh, key_of(st), k_end, b,
+                    p.num_blocks, lo, p.sinks);
     }
     cp_async_commit();
   }
@@ -716,10 +730,10 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
       const int tn = t + STAGES - 1;
       if (tn < n_tiles) {
         const int sn = tn % STAGES;
-        dec_load_tile(sK + sn * BN * D, p.kc, bt_row, p.block_size, p.nkv, kvh, k_begin + tn * BN, k_end, b,
-                      p.num_blocks);
-        dec_load_tile(sV + sn * BN * D, p.vc, bt_row, p.block_size, p.nkv, kvh, k_begin + tn * BN, k_end, b,
-                      p.num_blocks);
+        dec_load_tile<WIN>(sK + sn * BN * D, p.kc, bt_row, p.block_size, p.nkv, kvh, key_of(tn), k_end, b,
+                      p.num_blocks, lo, p.sinks);
+        dec_load_tile<WIN>(sV + sn * BN * D, p.vc, bt_row, p.block_size, p.nkv, kvh, key_of(tn), k_end, b,
+                      p.num_blocks, lo, p.sinks);
       }
       cp_async_commit();
     }
@@ -742,8 +756,8 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int key = k_begin + t * BN + warp * 16 + nt * 8 + (lane & 3) * 2 + (e & 1);
-        float v = key < k_end ? s[nt][e] * sl2 : -INFINITY;
+        const int key = key_of(t) + warp * 16 + nt * 8 + (lane & 3) * 2 + (e & 1);
+        float v = key < k_end && (!WIN || key >= lo || key < p.sinks) ? s[nt][e] * sl2 : -INFINITY;
         s[nt][e] = v;
         mx[e >> 1] = fmaxf(mx[e >> 1], v);
       }
@@ -841,9 +855,10 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
   }
 }
 
-__global__ void __launch_bounds__(NTHREADS, 3) decode_kernel(DecodeParams p) { decode_body<DEC_STAGES>(p); }
+__global__ void __launch_bounds__(NTHREADS, 3) decode_kernel(DecodeParams p) { decode_body<DEC_STAGES, false>(p); }
 // deeper ring (3 x 32 KB in flight per CTA) at 2 resident CTAs per SM
-__global__ void __launch_bounds__(NTHREADS, 2) decode_kernel_s3(DecodeParams p) { decode_body<3>(p); }
+__global__ void __launch_bounds__(NTHREADS, 2) decode_kernel_s3(DecodeParams p) { decode_body<3, false>(p); }
+__global__ void __launch_bounds__(NTHREADS, 2) decode_window_kernel(DecodeParams p) { decode_body<3, true>(p); }
 
 __global__ void decode_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_lse,
                                       bf16* __restrict__ o, int splits) {
@@ -1028,7 +1043,7 @@ int64_t decode_num_splits(int64_t batch, int64_t nkv, int64_t max_ctx) {
 // at least B*nq*splits*(D+1) elements used when splits > 1.
 at::Tensor attn_decode(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor block_table,
                        at::Tensor kv_lens, double scale, int64_t splits, c10::optional<at::Tensor> scratch,
-                       int64_t stages) {
+                       int64_t stages, int64_t window, int64_t sinks) {
   CHECK_CUDA_TENSOR(q);
   TORCH_CHECK(q.dim() == 3 && q.size(-1) == D, "q must be [B, heads, 128]");
   // rows may be strided (q viewed out of the fused qkv projection); heads and
@@ -1038,10 +1053,14 @@ at::Tensor attn_decode(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at:
               "q rows must hold contiguous heads and start 16-byte aligned");
   const int B = q.size(0), nq = q.size(1), nkv = k_cache.size(1);
   TORCH_CHECK(nq % nkv == 0 && nq / nkv <= 16, "GQA group must be <= 16");
+  TORCH_CHECK(window >= 0 && sinks >= 0 && window < (1 << 30) && sinks < (1 << 30),
+              "window and sinks must not be negative");
   at::cuda::CUDAGuard g(q.device());
   auto o = at::empty({B, nq, D}, q.options());
   if (B == 0) return o;
   DecodeParams p{};
+  p.window = (int)window;
+  p.sinks = (int)sinks;
   p.q = reinterpret_cast<const bf16*>(q.data_ptr());
   p.q_row = q.stride(0);
   p.kc = reinterpret_cast<const bf16*>(k_cache.data_ptr());
@@ -1069,11 +1088,16 @@ at::Tensor attn_decode(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at:
   }
   // ring depth: 3 stages x 2 CTAs/SM (default; 0.86-0.92 of copy bandwidth at
   // rollout shapes) or 2 stages x 3 CTAs/SM (stages == 2)
-  const int st = stages == 2 ? 2 : 3;
+  const int st = stages == 2 && window == 0 ? 2 : 3;
   const size_t sm = dec_smem(st);
-  ensure_smem_attr(st == 3 ? decode_kernel_s3 : decode_kernel, (int)sm);
+  if (window > 0)
+    ensure_smem_attr(decode_window_kernel, (int)sm);
+  else
+    ensure_smem_attr(st == 3 ? decode_kernel_s3 : decode_kernel, (int)sm);
   dim3 grid(B, nkv, splits);
-  if (st == 3)
+  if (window > 0)
+    decode_window_kernel<<<grid, NTHREADS, sm, stream()>>>(p);
+  else if (st == 3)
     decode_kernel_s3<<<grid, NTHREADS, sm, stream()>>>(p);
   else
     decode_kernel<<<grid, NTHREADS, sm, stream()>>>(p);

@@ -30,7 +30,15 @@ std::vector<at::Tensor> attn_varlen_bwd(at::Tensor dO, at::Tensor q, at::Tensor 
 int64_t decode_num_splits(int64_t batch, int64_t nkv, int64_t max_ctx);
 at::Tensor attn_decode(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor block_table,
                        at::Tensor kv_lens, double scale, int64_t splits, c10::optional<at::Tensor> scratch,
-                       int64_t stages);
+                       int64_t stages, int64_t window, int64_t sinks);
+at::Tensor attn_decode_fp8(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor k_scale, at::Tensor v_scale,
+                           at::Tensor block_table, at::Tensor kv_lens, double scale, int64_t window, int64_t sinks,
+                           at::Tensor err);
+at::Tensor rope_quant_kv(at::Tensor qkv, at::Tensor positions, at::Tensor cos_t, at::Tensor sin_t, int64_t nq,
+                         int64_t nkv, int64_t d, at::Tensor k_cache, at::Tensor v_cache, at::Tensor k_scale,
+                         at::Tensor v_scale, at::Tensor slots);
+void read_kv_cache(at::Tensor cache, at::Tensor scale, at::Tensor blocks, at::Tensor out,
+                   c10::optional<at::Tensor> out_blocks);
 std::tuple<pybind11::bytes, int64_t> ipc_handle(at::Tensor t);
 at::Tensor ipc_open(pybind11::bytes handle, int64_t offset, int64_t numel, at::ScalarType dtype, int64_t src_device);
 void enable_peer_access(int64_t peer);
@@ -100,7 +108,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_num_splits", &psrl::decode_num_splits);
   m.def("attn_decode", &psrl::attn_decode, pybind11::arg("q"), pybind11::arg("k_cache"), pybind11::arg("v_cache"),
         pybind11::arg("block_table"), pybind11::arg("kv_lens"), pybind11::arg("scale"), pybind11::arg("splits"), pybind11::arg("scratch"),
-        pybind11::arg("stages") = 0);
+        pybind11::arg("stages") = 0, pybind11::arg("window") = 0, pybind11::arg("sinks") = 0);
+  m.def("attn_decode_fp8", &psrl::attn_decode_fp8);
+  m.def("rope_quant_kv", &psrl::rope_quant_kv);
+  m.def("read_kv_cache", &psrl::read_kv_cache, py::arg("cache"), py::arg("scale"), py::arg("blocks"), py::arg("out"),
+        py::arg("out_blocks") = py::none());
   m.def("ipc_handle", &psrl::ipc_handle);
   m.def("ipc_open", &psrl::ipc_open);
   m.def("enable_peer_access", &psrl::enable_peer_access);

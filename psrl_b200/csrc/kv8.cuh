@@ -1,0 +1,74 @@
+// Shared pieces of the kernels that read the 8-bit paged KV cache (kv_fp8.cu
+// documents its format): argument checks, the TMA map over its pages and the
+// code conversions.
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+#include "driver_api.h"
+
+namespace psrl {
+namespace kv8 {
+
+// e4m3 codes in bytes 0 and 2 (even) or 1 and 3 (odd) of w as two f16 holding
+// the codes' values times 2^-8: sign to bit 15, exponent and mantissa to bits
+// 13..7.  Subnormal codes become subnormal f16 numbers, exactly.
+__device__ __forceinline__ uint32_t f16_odd(uint32_t w) { return (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u); }
+__device__ __forceinline__ uint32_t f16_even(uint32_t w) { return f16_odd(w << 8); }
+
+// 2^(byte - 127); byte 255 is a NaN, byte 0 (never written) counts as zero
+__device__ __forceinline__ float exp2_byte(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
+}
+
+// Tensor map over the codes: rows of 128 bytes (one vector each), boxes of
+// min(tile, block_size) rows, 128-byte swizzle.
+inline CUtensorMap map_codes(const at::Tensor& t, int tile) {
+  CUtensorMap m;
+  const cuuint64_t rows = (cuuint64_t)(t.size(0) * t.size(1) * t.size(2));
+  TORCH_CHECK(rows < (1ull << 31), "cache of more than 2^31 vectors");
+  cuuint64_t dims[2] = {128, rows};
+  cuuint64_t strides[1] = {128};
+  cuuint32_t box[2] = {128u, (cuuint32_t)std::min<int64_t>(tile, t.size(2))};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = PSRL_DRV(cuTensorMapEncodeTiled)(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, t.data_ptr(), dims, strides, box,
+                                                estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (", (int)r, ")");
+  return m;
+}
+
+// Checks shared by the attention entry points over a paged cache; k_scale and
+// v_scale undefined: a bf16 cache.
+inline void check_paged(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                        const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& block_table,
+                        const at::Tensor& kv_lens, int64_t B) {
+  const bool fp8 = k_scale.defined();
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes() && k_cache.size(3) == 128 &&
+                  k_cache.size(1) > 0 && k_cache.size(2) > 0,
+              "k_cache and v_cache must both be [blocks, nkv, block_size, 128]");
+  for (const at::Tensor* t : {&k_cache, &v_cache})
+    TORCH_CHECK(t->scalar_type() == (fp8 ? at::kFloat8_e4m3fn : at::kBFloat16) && t->is_contiguous() &&
+                    t->device() == q.device() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                "caches must be contiguous ", fp8 ? "float8_e4m3fn" : "bf16", " on q's device, 16-byte aligned");
+  if (fp8) {
+    for (const at::Tensor* t : {&k_scale, &v_scale})
+      TORCH_CHECK(t->scalar_type() == at::kByte && t->is_contiguous() && t->dim() == 3 &&
+                      t->size(0) == k_cache.size(0) && t->size(1) == k_cache.size(1) &&
+                      t->size(2) == k_cache.size(2) && t->device() == q.device() &&
+                      reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                  "exponents must be contiguous uint8 [blocks, nkv, block_size] on q's device, 16-byte aligned");
+  }
+  const int64_t bs = k_cache.size(2);
+  TORCH_CHECK(bs >= 16 && (bs & (bs - 1)) == 0, "block_size must be a power of two >= 16");
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == B &&
+                  (block_table.size(1) == 0 || block_table.stride(1) == 1) && block_table.device() == q.device(),
+              "block_table must be int32 [B, max_blocks] on q's device with unit inner stride");
+  TORCH_CHECK(kv_lens.scalar_type() == at::kInt && kv_lens.dim() == 1 && kv_lens.size(0) == B &&
+                  kv_lens.is_contiguous() && kv_lens.device() == q.device(),
+              "kv_lens must be int32 [B] on q's device");
+}
+
+}  // namespace kv8
+}  // namespace psrl

@@ -9,6 +9,7 @@ from .attention import (
     varlen_attention,
     varlen_attention_ref,
 )
+from .kv_quant import read_kv_cache, rope_quant_kv
 from .logprob import linear_logprob, linear_logprob_ref, logits_logprob
 from .norm import head_rms_norm, rms_norm, rms_norm_ref
 from .optim import NormAccumulator, adamw_, adamw_ref
@@ -17,7 +18,8 @@ from .sampling import sample, sample_ref
 
 __all__ = [
     "NormAccumulator", "adamw_", "adamw_ref", "check_kernel_bounds", "ext", "has_ext", "head_rms_norm", "kernel_checks_enabled", "linear_logprob",
-    "linear_logprob_ref", "logits_logprob", "paged_decode_attention", "paged_prefill_attention", "rms_norm",
-    "rms_norm_ref", "rope_qkv", "rope_qkv_", "rope_tables", "sample", "sample_ref", "swiglu", "swiglu_ref",
+    "linear_logprob_ref", "logits_logprob", "paged_decode_attention", "paged_prefill_attention",
+    "read_kv_cache", "rms_norm",
+    "rms_norm_ref", "rope_qkv", "rope_qkv_", "rope_quant_kv", "rope_tables", "sample", "sample_ref", "swiglu", "swiglu_ref",
     "varlen_attention", "varlen_attention_ref",
 ]

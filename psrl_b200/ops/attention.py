@@ -50,8 +50,47 @@ def gather_paged_kv(k_cache, v_cache, block_table_row, length):
     return k, v
 
 
-def paged_attention_ref(q, k_cache, v_cache, cu_q, kv_lens, block_table, scale):
+def window_mask(qpos, kpos, window=None, sinks=0):
+    """True where the query at ``qpos`` sees the key at ``kpos``: causal, and with
+    a ``window`` only the last ``window`` positions and the first ``sinks``."""
+    ok = kpos <= qpos
+    if window:
+        ok = ok & ((qpos - kpos < window) | (kpos < sinks))
+    return ok
+
+
+def _masked_softmax(att, ok):
+    """Softmax over the kept scores; a row that keeps none gives zeros."""
+    return torch.where(ok, att.masked_fill(~ok, float("-inf")).softmax(-1), torch.zeros((), dtype=att.dtype,
+                                                                                         device=att.device))
+
+
+def _window_args(window, sinks):
+    """(window or 0, sinks) checked: a window is a positive number of positions."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window (without one every earlier position is visible)")
+        return 0, 0
+    if int(window) < 1 or int(sinks) < 0:
+        raise ValueError(f"window must be >= 1 and sinks >= 0, not {window} and {sinks}")
+    return int(window), int(sinks)
+
+
+def _paged_args(q, k_cache, v_cache, k_scale, v_scale):
+    if (k_scale is None) != (v_scale is None):
+        raise ValueError("an 8-bit cache needs both k_scale and v_scale")
+    want = torch.bfloat16 if k_scale is None else torch.float8_e4m3fn
+    if q.is_cuda and (k_cache.dtype != want or v_cache.dtype != want):
+        raise ValueError(f"caches of {k_cache.dtype} and {v_cache.dtype} {'with' if k_scale is not None else 'without'} "
+                         "exponent bytes: an 8-bit cache is float8_e4m3fn with k_scale and v_scale")
+
+
+def paged_attention_ref(q, k_cache, v_cache, cu_q, kv_lens, block_table, scale, k_scale=None, v_scale=None,
+                        window=None, sinks=0):
     """Queries are the last q_len positions of each context (causal)."""
+    if k_scale is not None:
+        from .kv_quant import dequantise_ref
+        k_cache, v_cache = dequantise_ref(k_cache, k_scale), dequantise_ref(v_cache, v_scale)
     T, nq, d = q.shape
     nkv = k_cache.shape[1]
     g = nq // nkv
@@ -71,8 +110,9 @@ def paged_attention_ref(q, k_cache, v_cache, cu_q, kv_lens, block_table, scale):
         ql = e - s
         qpos = torch.arange(L - ql, L, device=q.device)[:, None]
         kpos = torch.arange(L, device=q.device)[None, :]
-        att = att.masked_fill(kpos > qpos, float("-inf")).softmax(-1)
-        out[s:e] = (att @ vs).transpose(0, 1).to(q.dtype)
+        ok = window_mask(qpos, kpos, window, sinks)
+        vs = vs.masked_fill(~ok.any(0)[None, :, None], 0.0)
+        out[s:e] = (_masked_softmax(att, ok) @ vs).transpose(0, 1).to(q.dtype)
     return out
 
 
@@ -149,13 +189,27 @@ def _ref_autograd(q, k, v, cu_seqlens, scale):
     return torch.cat(outs, 0) if outs else q.new_zeros(0, nq, d)
 
 
-def paged_prefill_attention(q, k_cache, v_cache, cu_q, kv_lens, block_table, max_q_len, scale=None):
-    """q [T, nq, d] (view ok); returns [T, nq, d]."""
+def paged_prefill_attention(q, k_cache, v_cache, cu_q, kv_lens, block_table, max_q_len, scale=None, k_scale=None,
+                            v_scale=None, window=None, sinks=0):
+    """A chunk of new tokens per sequence against its paged context, which holds
+    the chunk's own keys already: q [T, nq, d] (view ok), sequence b's queries
+    [cu_q[b], cu_q[b+1]) being its last positions; returns [T, nq, d].
+
+    ``k_scale`` / ``v_scale``: exponent bytes of an 8-bit cache (:mod:`.kv_quant`).
+    ``window`` / ``sinks``: see :func:`window_mask`."""
     d = q.shape[-1]
     scale = scale if scale is not None else 1.0 / math.sqrt(d)
+    win, sinks = _window_args(window, sinks)
+    _paged_args(q, k_cache, v_cache, k_scale, v_scale)
     if q.is_cuda and d == 128:
-        return ext().attn_paged_prefill(q, k_cache, v_cache, cu_q, kv_lens, block_table, int(max_q_len), scale)
-    return paged_attention_ref(q, k_cache, v_cache, cu_q, kv_lens, block_table, scale)
+        if k_scale is None and not win:
+            return ext().attn_paged_prefill(q, k_cache, v_cache, cu_q, kv_lens, block_table, int(max_q_len), scale)
+        from .gemm import _err
+        if not (q.stride(2) == 1 and q.stride(1) % 8 == 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0):
+            q = q.contiguous()
+        return ext().attn_paged_chunk(q, k_cache, v_cache, k_scale, v_scale, cu_q, kv_lens, block_table,
+                                      int(max_q_len), scale, win, sinks, _err(q.device))
+    return paged_attention_ref(q, k_cache, v_cache, cu_q, kv_lens, block_table, scale, k_scale, v_scale, window, sinks)
 
 
 def decode_splits(batch: int, nkv: int, max_ctx: int) -> int:
@@ -163,19 +217,33 @@ def decode_splits(batch: int, nkv: int, max_ctx: int) -> int:
 
 
 def paged_decode_attention(q, k_cache, v_cache, block_table, kv_lens, scale=None, splits: int | None = None,
-                           scratch: torch.Tensor | None = None, stages: int = 0):
-    """q [B, nq, d] -> [B, nq, d]; kv_lens include the current token."""
+                           scratch: torch.Tensor | None = None, stages: int = 0, k_scale=None, v_scale=None,
+                           window: int | None = None, sinks: int = 0):
+    """One new token per sequence against its paged context: q [B, nq, d] ->
+    [B, nq, d]; kv_lens include the current token.
+
+    ``k_scale`` / ``v_scale``: exponent bytes of an 8-bit cache (:mod:`.kv_quant`),
+    whose kernel shares the work out by itself (``splits``, ``scratch`` and
+    ``stages`` do not apply).  ``window`` / ``sinks``: see :func:`window_mask`."""
     d = q.shape[-1]
     scale = scale if scale is not None else 1.0 / math.sqrt(d)
+    win, sinks = _window_args(window, sinks)
+    _paged_args(q, k_cache, v_cache, k_scale, v_scale)
     if q.is_cuda and d == 128:
-        if splits is None:
-            splits = decode_splits(q.shape[0], k_cache.shape[1], int(block_table.shape[1] * k_cache.shape[2]))
         if not (q.stride(2) == 1 and q.stride(1) == d and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0):
             q = q.contiguous()
-        return ext().attn_decode(q, k_cache, v_cache, block_table, kv_lens, scale, int(splits), scratch, int(stages))
+        if k_scale is not None:
+            from .gemm import _err
+            return ext().attn_decode_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, kv_lens, scale, win,
+                                         sinks, _err(q.device))
+        if splits is None:
+            ctx = int(block_table.shape[1] * k_cache.shape[2])
+            splits = decode_splits(q.shape[0], k_cache.shape[1], min(ctx, win + sinks) if win else ctx)
+        return ext().attn_decode(q, k_cache, v_cache, block_table, kv_lens, scale, int(splits), scratch, int(stages),
+                                 win, sinks)
     B = q.shape[0]
     cu = torch.arange(B + 1, dtype=torch.int32, device=q.device)
-    return paged_attention_ref(q, k_cache, v_cache, cu, kv_lens, block_table, scale)
+    return paged_attention_ref(q, k_cache, v_cache, cu, kv_lens, block_table, scale, k_scale, v_scale, window, sinks)
 
 
 # ------------------------------------------- queries against separate keys
