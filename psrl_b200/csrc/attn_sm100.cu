@@ -28,6 +28,13 @@
 // 0 .. p + Lk - Lq.  Context-parallel attention uses this for a rank's query
 // chunks against the gathered keys of the sequence prefix.
 //
+// Sliding window (WIN): row p sees the keys with p + off - key < window, and the
+// first `sinks` keys.  The block's key tiles are then the sinks' tiles [0, ns)
+// and the window's, from w0 on; tile B skips the first of those where its window
+// starts a tile later.  Only tiles that cross a limit are masked, so a window
+// costs (window + 256 or so) / length of the causal time: measured forward, 32
+// heads, 16384 tokens: see the table of figures at the launcher.
+//
 // Work per block: tile A needs the key tiles up to its last row's limit,
 // tile B one more or two; only tiles that cross a row's limit are masked.  Blocks are launched
 // largest first.  Every wait is bounded; on timeout the kernel records an
@@ -67,6 +74,7 @@ struct FwdArgs {
   bf16* o;           // [T, nq * D]
   int64_t o_row;
   float* lse;        // [nq, T] natural log, or null
+  int window, sinks; // WIN only
   int* err;
 };
 
@@ -81,6 +89,19 @@ __device__ __forceinline__ void set_err(int* err, int code, int it = -1) {
   }
 }
 
+// Rows [row0, rows) of a tile (two 64-column atoms of `rows` rows) become zeros,
+// by threads tid of n.  Rows behind a sequence's end belong to the next sequence
+// or to nobody; whatever they hold, times a probability of zero, must add zero,
+// which a NaN would not.  The caller orders the writes (fence_async_smem, then
+// its arrive) before the MMA that reads the tile.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int row0, int rows, int tid, int n) {
+  for (int i = tid; i < (rows - row0) * 16; i += n) {
+    const int atom = i & 1, c = (i >> 1) & 7, r = row0 + (i >> 4);
+    *reinterpret_cast<uint4*>(tile + atom * rows * 128 + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <bool WIN>
 __global__ void __launch_bounds__(NTHREADS, 1)
     fa_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV, FwdArgs a) {
   const int h = blockIdx.x, b = blockIdx.y;
@@ -89,12 +110,29 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   const int sk0 = a.cu_k[b], Lk = a.cu_k[b + 1] - sk0;
   const int off = Lk - L;  // query row p sees keys 0 .. p + off
   const int q0 = blk * 2 * BQ;
+  if constexpr (WIN) {
+    // rows behind the last sequence are zeros
+    if (b == (int)gridDim.y - 1 && blockIdx.z == 0)
+      for (int64_t i = (int64_t)a.cu[gridDim.y] * (D / 8) + threadIdx.x; i < (int64_t)a.T * (D / 8); i += NTHREADS)
+        *reinterpret_cast<uint4*>(a.o + (i / (D / 8)) * a.o_row + (int64_t)h * D + (i % (D / 8)) * 8) =
+            make_uint4(0, 0, 0, 0);
+  }
   if (q0 >= L) return;  // uniform for the whole CTA, before any barrier
   const int rowsB = max(0, min(BQ, L - q0 - BQ));
   const int nKt = (Lk + BKV - 1) / BKV;
-  const int nA = min(nKt, (min(q0 + BQ, L) - 1 + off) / BKV + 1);
-  const int nB = rowsB > 0 ? min(nKt, (q0 + BQ + rowsB - 1 + off) / BKV + 1) : 0;
+  // list of key tiles: index j is tile j below ns, tile j + gap from there on
+  const int w0 = WIN ? max(0, q0 + off - a.window + 1) / BKV : 0;
+  const int ns = WIN ? min((a.sinks + BKV - 1) / BKV, w0) : 0;
+  const int gap = w0 - ns;
+  // tile B leaves out the list's entries [ns, ns + skip): before its window
+  // (unless that tile, w0, holds sinks)
+  const int skip = WIN && w0 * BKV >= a.sinks ? max(0, q0 + BQ + off - a.window + 1) / BKV - w0 : 0;
+  const int nA = min(nKt, (min(q0 + BQ, L) - 1 + off) / BKV + 1) - gap;
+  const int nB = rowsB > 0 ? min(nKt, (q0 + BQ + rowsB - 1 + off) / BKV + 1) - gap : 0;
   const int nK = max(nA, nB);
+  auto key_tile = [&](int j) { return !WIN || j < ns ? j : j + gap; };
+  auto in_b = [&](int j) { return j < nB && (!WIN || j < ns || j >= ns + skip); };
+  auto count_b = [&](int j) { return !WIN || j < ns ? j : j - skip; };  // tiles of B before list entry j
   const int hk = h / (a.nq / a.nkv);
   const int xq = a.q_col + h * D, xk = a.k_col + hk * D, xv = a.v_col + hk * D;
 
@@ -155,7 +193,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         const uint32_t fb = bkf + 8 * st;
         mbar_expect_tx(fb, STAGE);
         const uint32_t sk = smem_u32(smem + OFF_KV + st * STAGE), sv = sk + KV_TILE;
-        const int y = sk0 + j * BKV;
+        const int y = sk0 + key_tile(j) * BKV;
         tma_load_2d(sk, &tmKV, xk, y, fb);
         tma_load_2d(sk + ATOM, &tmKV, xk + 64, y, fb);
         tma_load_2d(sv, &tmKV, xv, y, fb);
@@ -187,35 +225,35 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
         commit_1cta(bsf + 8 * g);
       };
-      auto issue_pv = [&](int g, int j) {
+      auto issue_pv = [&](int g, int j, bool first) {
         fence_after();
         const uint32_t sv = smem_u32(smem + OFF_KV + (j % NS) * STAGE + KV_TILE);
 #pragma unroll
         for (int k = 0; k < BKV / 16; ++k)
-          mma_1cta_ts(tO(g), tS(g) + k * 8, desc_sw128(sv + k * 2048, ATOM, 1024), idesc_pv, (j > 0 || k > 0));
+          mma_1cta_ts(tO(g), tS(g) + k * 8, desc_sw128(sv + k * 2048, ATOM, 1024), idesc_pv, (!first || k > 0));
       };
       wait_kv(0);
       if (ok) {
         issue_s(0, 0);
-        if (nB) issue_s(1, 0);
+        if (in_b(0)) issue_s(1, 0);
       }
       int where = ok ? 0 : 120;
       for (int j = 0; j < nK && ok && !s_abort; ++j) {
         if (j < nA) {
           if (!mbar_wait(bpf, j & 1)) { ok = false; where = 121 + 1000 * j; break; }
-          issue_pv(0, j);
+          issue_pv(0, j, j == 0);
         }
         if (j + 1 < nA) {
           wait_kv(j + 1);
           if (!ok) { where = 122 + 1000 * j; break; }
           issue_s(0, j + 1);
         }
-        if (j < nB) {
-          if (!mbar_wait(bpf + 8, j & 1)) { ok = false; where = 123 + 1000 * j; break; }
-          issue_pv(1, j);
+        if (in_b(j)) {
+          if (!mbar_wait(bpf + 8, count_b(j) & 1)) { ok = false; where = 123 + 1000 * j; break; }
+          issue_pv(1, j, count_b(j) == 0);
         }
         commit_1cta(bke + 8 * (j % NS));  // K_j / V_j no longer read
-        if (j + 1 < nB) {
+        if (in_b(j + 1)) {
           wait_kv(j + 1);
           if (!ok) { where = 124 + 1000 * j; break; }
           issue_s(1, j + 1);
@@ -230,7 +268,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   } else {
     // -------------------------------------------------------------- softmax
     const int g = (warp - 2) >> 2;  // 0: tile A (warps 2..5), 1: tile B (warps 6..9)
-    const int n = g == 0 ? nA : nB;
+    const int n = g == 0 ? nA : (nB > 0 ? count_b(nB) : 0);
     const int quad = warp & 3;
     const int r = quad * 32 + lane;           // row within the tile
     const int row_pos = q0 + g * BQ + r;      // position within the sequence
@@ -244,8 +282,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         break;
       }
       fence_after();
-      const int lim = row_pos + off - j * BKV;  // last key column of tile j this row sees
-      const bool masked_tile = __any_sync(0xffffffffu, lim < BKV - 1);
+      const int key0 = (WIN ? key_tile(g == 0 || j < ns ? j : j + skip) : j) * BKV;
+      if (WIN && key0 + BKV > Lk) {
+        const int jj = g == 0 || j < ns ? j : j + skip;
+        mbar_wait(bkf + 8 * (jj % NS), (jj / NS) & 1);  // complete: S of this tile is
+        zero_rows(smem + OFF_KV + (jj % NS) * STAGE + KV_TILE, Lk - key0, BKV, r, 128);
+        fence_async_smem();
+      }
+      const int lim = row_pos + off - key0;  // last key column of the tile this row sees
+      const int lo = lim - a.window + 1, sk = a.sinks - key0;  // WIN: columns from lo on, and those before sk
+      const bool masked_tile = __any_sync(0xffffffffu, lim < BKV - 1 || (WIN && lo > 0 && sk < BKV));
       // the whole S row (128 fp32 columns) comes out of TMEM in four loads
       // behind one wait and stays in registers for both passes
       uint32_t v[128];
@@ -257,7 +303,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       if (masked_tile) {
 #pragma unroll
         for (int i = 0; i < 128; ++i)
-          if (i > lim) v[i] = 0xff800000u;  // -inf: key past this row's causal limit
+          if (i > lim || (WIN && i < lo && i >= sk)) v[i] = 0xff800000u;  // -inf: a key this row does not see
       }
       // pass 1: row maximum of the raw scores; the scale is positive, so it is
       // applied once, to the maximum
@@ -393,16 +439,27 @@ struct BwdArgs {
   int hsplit;
   float* part;
   int64_t part_rows;
+  int window, sinks;  // WIN only
   int* err;
 };
 
 __global__ void fa_bwd_dot(const bf16* __restrict__ o, const bf16* __restrict__ dout, int64_t T, int nq,
-                           float* __restrict__ dd) {
+                           float* __restrict__ dd, const int* __restrict__ cu_end, bf16* __restrict__ dq,
+                           int64_t dq_row, int dq_col, bf16* __restrict__ dkv, int64_t dkv_row, int dkv_cols) {
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (w >= T * nq) return;
   const int64_t t = w / nq;
   const int h = (int)(w - t * nq);
+  if (cu_end && t >= *cu_end) {
+    // a row behind the last sequence: its gradients are zeros (head 0's warp also
+    // clears the key and value columns where they lie in the same tensor)
+    *reinterpret_cast<uint2*>(dq + t * dq_row + dq_col + (int64_t)h * D + lane * 4) = make_uint2(0, 0);
+    if (h == 0)
+      for (int c = lane * 4; c < dkv_cols; c += 128)
+        *reinterpret_cast<uint2*>(dkv + t * dkv_row + c) = make_uint2(0, 0);
+    return;
+  }
   const bf16* po = o + w * D + lane * 4;
   const bf16* pd = dout + w * D + lane * 4;
   float s = 0.f;
@@ -462,6 +519,7 @@ constexpr int OFF_DKV_STAGE = 2 * KV_TILE;               // after the resident K
 constexpr int OFF_DKV_BAR = OFF_DKV_STAGE + NSK * DKV_STAGE;
 constexpr int SMEM_DKV = OFF_DKV_BAR + 256 + 1024;
 
+template <bool WIN>
 __global__ void __launch_bounds__(NT_BWD, 1)
     fa_bwd_dkdv(const __grid_constant__ CUtensorMap tmQ64, const __grid_constant__ CUtensorMap tmKV,
                 const __grid_constant__ CUtensorMap tm_do64, BwdArgs a) {
@@ -472,9 +530,14 @@ __global__ void __launch_bounds__(NT_BWD, 1)
   const int off = Lk - L;
   if (j * BKV >= Lk) return;
   const int G = a.nq / a.nkv, Gc = G / a.hsplit;
-  const int nqt = (L + BQ2 - 1) / BQ2;
   const int i0 = max(0, j * BKV - off) / BQ2;  // first 64-row query tile that sees key tile j
-  const int per_head = nqt - i0;
+  int nqt = (L + BQ2 - 1) / BQ2;
+  // WIN: the last query that sees a key is window - 1 after it, unless it is a sink
+  if (WIN && j * BKV >= a.sinks) {
+    const int64_t last = (int64_t)j * BKV + BKV - 1 + a.window - 1 - off;
+    nqt = last < 0 ? 0 : (int)min((int64_t)nqt, last / BQ2 + 1);
+  }
+  const int per_head = max(0, nqt - i0);
   const int iters = Gc * per_head;
   const int xk = a.k_col + hk * D, xv = a.v_col + hk * D;
 
@@ -646,7 +709,15 @@ __global__ void __launch_bounds__(NT_BWD, 1)
       const float* dd_s = lse_s + BQ2;
       // every query of tile i is in the sequence and sees every key of tile j:
       // no per-element mask
-      const bool full = (i + 1) * BQ2 <= L && (j + 1) * BKV - 1 <= i * BQ2 + off;
+      const bool full = (i + 1) * BQ2 <= L && (j + 1) * BKV - 1 <= i * BQ2 + off &&
+                        (!WIN || (i + 1) * BQ2 - 1 + off - j * BKV < a.window || (j + 1) * BKV <= a.sinks);
+      if (WIN && (i + 1) * BQ2 > L) {
+        mbar_wait(bsf0 + 8 * st, (it / NSK) & 1);  // complete: S^T of this step is
+        uint8_t* stg = smem + OFF_DKV_STAGE + st * DKV_STAGE;
+        zero_rows(stg, L - i * BQ2, BQ2, threadIdx.x - 64, 256);
+        zero_rows(stg + KV64_TILE, L - i * BQ2, BQ2, threadIdx.x - 64, 256);
+        fence_async_smem();
+      }
       uint32_t vs[32], vp[32], pk[16], dk[16];
       tmem_ld32(tS(bb) + lane_off + col0, vs);
       tmem_ld32(tP(bb) + lane_off + col0, vp);
@@ -657,7 +728,10 @@ __global__ void __launch_bounds__(NT_BWD, 1)
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const int q = i * BQ2 + col0 + e;
-          if (!(q < L && key <= q + off)) vs[e] = 0xff800000u;
+          if (!(q < L && key <= q + off && (!WIN || q + off - key < a.window || key < a.sinks))) {
+            vs[e] = 0xff800000u;
+            if (WIN) vp[e] = 0;
+          }
         }
       }
 #pragma unroll
@@ -703,6 +777,11 @@ __global__ void __launch_bounds__(NT_BWD, 1)
         tmem_ld32(tdV + lane_off + col0, vdv);
         tmem_ld32(tdK + lane_off + col0, vdk);
         tmem_wait_ld();
+        if (WIN && iters == 0) {
+          // no query sees these keys: nothing was accumulated
+#pragma unroll
+          for (int e = 0; e < 32; ++e) vdv[e] = vdk[e] = 0;
+        }
         if (valid && a.hsplit > 1) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
@@ -736,6 +815,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
 }
 
 
+template <bool WIN>
 __global__ void __launch_bounds__(NT_BWD, 1)
     fa_bwd_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV64,
               const __grid_constant__ CUtensorMap tm_do, BwdArgs a) {
@@ -745,7 +825,11 @@ __global__ void __launch_bounds__(NT_BWD, 1)
   const int sk0 = a.cu_k[b], Lk = a.cu_k[b + 1] - sk0;
   const int off = Lk - L;
   if (i * BQ >= L) return;
-  const int n = min((Lk + BK2 - 1) / BK2, (min((i + 1) * BQ, L) - 1 + off) / BK2 + 1);
+  // WIN: the sinks' key tiles [0, ns), then those from the first row's window on
+  const int w0 = WIN ? max(0, i * BQ + off - a.window + 1) / BK2 : 0;
+  const int ns = WIN ? min((a.sinks + BK2 - 1) / BK2, w0) : 0;
+  const int n = min((Lk + BK2 - 1) / BK2, (min((i + 1) * BQ, L) - 1 + off) / BK2 + 1) - (w0 - ns);
+  auto key_tile = [&](int jj) { return !WIN || jj < ns ? jj : jj - ns + w0; };
   const int hk = h / (a.nq / a.nkv);
   const int xk = a.k_col + hk * D, xv = a.v_col + hk * D;
 
@@ -805,7 +889,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
         const uint32_t fb = bkf0 + 8 * st;
         mbar_expect_tx(fb, DQ_STAGE);
         const uint32_t sk = smem_u32(smem + OFF_DQ_KV + st * DQ_STAGE), sv = sk + KV64_TILE;
-        const int y2 = sk0 + jj * BK2;
+        const int y2 = sk0 + key_tile(jj) * BK2;
         tma_load_2d(sk, &tmKV64, xk, y2, fb);
         tma_load_2d(sk + ATOM64, &tmKV64, xk + 64, y2, fb);
         tma_load_2d(sv, &tmKV64, xv, y2, fb);
@@ -891,7 +975,14 @@ __global__ void __launch_bounds__(NT_BWD, 1)
       }
       fence_after();
       // every query of tile i is in the sequence and sees every key of tile jj
-      const bool full = (i + 1) * BQ <= L && (jj + 1) * BK2 - 1 <= i * BQ + off;
+      const int key0 = key_tile(jj) * BK2;
+      const bool full = (i + 1) * BQ <= L && key0 + BK2 - 1 <= i * BQ + off &&
+                        (!WIN || (i + 1) * BQ - 1 + off - key0 < a.window || key0 + BK2 <= a.sinks);
+      if (WIN && key0 + BK2 > Lk) {
+        mbar_wait(bkf0 + 8 * (jj % NSQ), (jj / NSQ) & 1);  // complete: S of this tile is
+        zero_rows(smem + OFF_DQ_KV + (jj % NSQ) * DQ_STAGE, Lk - key0, BK2, threadIdx.x - 64, 256);
+        fence_async_smem();
+      }
       uint32_t vs[32], vp[32], dk[16];
       tmem_ld32(tS(bb) + lane_off + col0, vs);
       tmem_ld32(tP(bb) + lane_off + col0, vp);
@@ -900,8 +991,11 @@ __global__ void __launch_bounds__(NT_BWD, 1)
         // masked scores become -inf, so P = 0 and dS = P (dP - D) = 0
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const int key = jj * BK2 + col0 + e;
-          if (!(qin && key <= q + off)) vs[e] = 0xff800000u;
+          const int key = key0 + col0 + e;
+          if (!(qin && key <= q + off && (!WIN || q + off - key < a.window || key < a.sinks))) {
+            vs[e] = 0xff800000u;
+            if (WIN) vp[e] = 0;
+          }
         }
       }
 #pragma unroll
@@ -978,8 +1072,11 @@ static CUtensorMap map_rows_64x128(const at::Tensor& t) { return map_rows_64xR(t
 // are the last of its key rows [cu_k[b], cu_k[b+1]).
 static std::vector<at::Tensor> fwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& cu_q,
                                           const at::Tensor& cu_k, int64_t max_q, int64_t nq, int64_t nkv, int q_col,
-                                          int k_col, int v_col, double scale, bool want_lse, const at::Tensor& err) {
+                                          int k_col, int v_col, double scale, bool want_lse, const at::Tensor& err,
+                                          int64_t window, int64_t sinks) {
   CHECK_DTYPE(q, at::kBFloat16);
+  TORCH_CHECK(window >= 0 && sinks >= 0 && window < (1 << 30) && sinks < (1 << 30),
+              "window and sinks must not be negative");
   CHECK_DTYPE(kv, at::kBFloat16);
   TORCH_CHECK(nq % nkv == 0, "nq must be a multiple of nkv");
   TORCH_CHECK(cu_q.scalar_type() == at::kInt && cu_q.is_contiguous() && cu_k.scalar_type() == at::kInt &&
@@ -990,7 +1087,7 @@ static std::vector<at::Tensor> fwd_launch(const at::Tensor& q, const at::Tensor&
   at::cuda::CUDAGuard g(q.device());
   auto o = at::empty({T, nq * D}, q.options());
   auto lse = want_lse ? at::empty({nq, T}, q.options().dtype(at::kFloat)) : at::Tensor();
-  if (T == 0 || B <= 0 || max_q <= 0) return {o, lse};
+  if (T == 0 || B <= 0 || max_q <= 0) return {window > 0 ? o.zero_() : o, lse};
   const CUtensorMap tq = map_rows_64x128(q), tkv = map_rows_64x128(kv);
   FwdArgs a{};
   a.cu = cu_q.data_ptr<int>();
@@ -1007,9 +1104,12 @@ static std::vector<at::Tensor> fwd_launch(const at::Tensor& q, const at::Tensor&
   a.o_row = nq * D;
   a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
   a.err = err.data_ptr<int>();
-  ensure_smem_attr(fa_fwd_kernel, SMEM_BYTES);
+  a.window = (int)window;
+  a.sinks = (int)sinks;
+  auto* kern = window > 0 ? fa_fwd_kernel<true> : fa_fwd_kernel<false>;
+  ensure_smem_attr(kern, SMEM_BYTES);
   dim3 grid((unsigned)nq, (unsigned)B, (unsigned)a.blocks_z);
-  fa_fwd_kernel<<<grid, NTHREADS, SMEM_BYTES, stream()>>>(tq, tkv, a);
+  kern<<<grid, NTHREADS, SMEM_BYTES, stream()>>>(tq, tkv, a);
   PSRL_CHECK_LAUNCH();
   return {o, lse};
 }
@@ -1018,12 +1118,13 @@ static std::vector<at::Tensor> fwd_launch(const at::Tensor& q, const at::Tensor&
 // token, unit inner stride, rows on 16-byte boundaries).  Returns
 // {o [T, nq * 128] bf16, lse [nq, T] fp32 (natural log; empty unless want_lse)}.
 std::vector<at::Tensor> attn_fwd_sm100(at::Tensor qkv, at::Tensor cu_seqlens, int64_t max_seqlen, int64_t nq,
-                                       int64_t nkv, double scale, bool want_lse, at::Tensor err) {
+                                       int64_t nkv, double scale, bool want_lse, at::Tensor err, int64_t window,
+                                          int64_t sinks) {
   CHECK_CUDA_TENSOR(qkv);
   TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) == (nq + 2 * nkv) * D,
               "qkv must be [T, (nq + 2 nkv) * 128] with unit inner stride");
   return fwd_launch(qkv, qkv, cu_seqlens, cu_seqlens, max_seqlen, nq, nkv, 0, (int)(nq * D), (int)((nq + nkv) * D),
-                    scale, want_lse, err);
+                    scale, want_lse, err, window, sinks);
 }
 
 // Queries against separately stored keys / values (context parallelism):
@@ -1032,11 +1133,12 @@ std::vector<at::Tensor> attn_fwd_sm100(at::Tensor qkv, at::Tensor cu_seqlens, in
 // the last of its cu_k[b+1] - cu_k[b] (>=) key positions.
 std::vector<at::Tensor> attn_fwd_sm100_kv(at::Tensor q, at::Tensor kv, at::Tensor cu_q, at::Tensor cu_k,
                                           int64_t max_q, int64_t nq, int64_t nkv, double scale, bool want_lse,
-                                          at::Tensor err) {
+                                          at::Tensor err, int64_t window,
+                                          int64_t sinks) {
   CHECK_CUDA_TENSOR(q);
   TORCH_CHECK(q.dim() == 2 && q.size(1) >= nq * D && kv.dim() == 2 && kv.size(1) == 2 * nkv * D,
               "q [Tq, nq * 128], kv [Tk, 2 nkv * 128]");
-  return fwd_launch(q, kv, cu_q, cu_k, max_q, nq, nkv, 0, 0, (int)(nkv * D), scale, want_lse, err);
+  return fwd_launch(q, kv, cu_q, cu_k, max_q, nq, nkv, 0, 0, (int)(nkv * D), scale, want_lse, err, window, sinks);
 }
 
 // Shared backward launcher (see fwd_launch); writes dq rows into `dq` and dk /
@@ -1044,7 +1146,8 @@ std::vector<at::Tensor> attn_fwd_sm100_kv(at::Tensor q, at::Tensor kv, at::Tenso
 static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& o, const at::Tensor& dout,
                        const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k, int64_t max_q,
                        int64_t max_k, int64_t nq, int64_t nkv, int q_col, int k_col, int v_col, double scale,
-                       at::Tensor& dq, int dq_col, at::Tensor& dkv, int dk_col, int dv_col, const at::Tensor& err) {
+                       at::Tensor& dq, int dq_col, at::Tensor& dkv, int dk_col, int dv_col, const at::Tensor& err,
+                       int64_t window, int64_t sinks) {
   CHECK_DTYPE(q, at::kBFloat16);
   CHECK_DTYPE(kv, at::kBFloat16);
   CHECK_DTYPE(o, at::kBFloat16);
@@ -1057,11 +1160,14 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
   const int B = (int)cu_q.numel() - 1;
   if (T == 0 || B <= 0 || max_q <= 0) return;
   auto dd = at::empty({nq, T}, q.options().dtype(at::kFloat));
+  const bool same = dq.data_ptr() == dkv.data_ptr();  // one [q | k | v] gradient
   {
     const int64_t warps = T * nq;
     fa_bwd_dot<<<(unsigned)((warps * 32 + 255) / 256), 256, 0, stream()>>>(
         reinterpret_cast<const bf16*>(o.data_ptr()), reinterpret_cast<const bf16*>(dout.data_ptr()), T, (int)nq,
-        dd.data_ptr<float>());
+        dd.data_ptr<float>(), window > 0 ? cu_q.data_ptr<int>() + B : nullptr, reinterpret_cast<bf16*>(dq.data_ptr()),
+        dq.stride(0), dq_col, same ? reinterpret_cast<bf16*>(dkv.data_ptr()) + dk_col : nullptr, dkv.stride(0),
+        same ? (int)(2 * nkv * D) : 0);
     PSRL_CHECK_LAUNCH();
   }
   const CUtensorMap tq = map_rows_64x128(q), tkv = map_rows_64x128(kv), tdo = map_rows_64x128(dout.view({T, nq * D}));
@@ -1087,8 +1193,12 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
   a.dk_col = dk_col;
   a.dv_col = dv_col;
   a.err = err.data_ptr<int>();
-  ensure_smem_attr(fa_bwd_dkdv, SMEM_DKV);
-  ensure_smem_attr(fa_bwd_dq, SMEM_DQ);
+  a.window = (int)window;
+  a.sinks = (int)sinks;
+  auto* kern_dkdv = window > 0 ? fa_bwd_dkdv<true> : fa_bwd_dkdv<false>;
+  auto* kern_dq = window > 0 ? fa_bwd_dq<true> : fa_bwd_dq<false>;
+  ensure_smem_attr(kern_dkdv, SMEM_DKV);
+  ensure_smem_attr(kern_dq, SMEM_DQ);
   const unsigned kz = (unsigned)((max_k + BKV - 1) / BKV);
   // Causal balance: the CTA of key tile 0 loops over every query tile of all
   // G = nq / nkv heads, the last key tile over one.  Split the heads of each
@@ -1109,8 +1219,8 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
     a.part_rows = kv.size(0);
   }
   const CUtensorMap tq64 = map_rows_64xR(q, 64u), tdo64 = map_rows_64xR(dout.view({T, nq * D}), 64u);
-  fa_bwd_dkdv<<<dim3((unsigned)nkv, (unsigned)B, kz * (unsigned)hsplit), NT_BWD, SMEM_DKV, stream()>>>(tq64, tkv,
-                                                                                                       tdo64, a);
+  kern_dkdv<<<dim3((unsigned)nkv, (unsigned)B, kz * (unsigned)hsplit), NT_BWD, SMEM_DKV, stream()>>>(tq64, tkv, tdo64,
+                                                                                                     a);
   PSRL_CHECK_LAUNCH();
   if (hsplit > 1) {
     const int64_t threads = kv.size(0) * nkv * 2 * D / 8;
@@ -1119,14 +1229,15 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
     PSRL_CHECK_LAUNCH();
   }
   const CUtensorMap tkv64 = map_rows_64xR(kv, 64u);
-  fa_bwd_dq<<<dim3((unsigned)nq, (unsigned)B, (unsigned)a.blocks_z), NT_BWD, SMEM_DQ, stream()>>>(tq, tkv64, tdo, a);
+  kern_dq<<<dim3((unsigned)nq, (unsigned)B, (unsigned)a.blocks_z), NT_BWD, SMEM_DQ, stream()>>>(tq, tkv64, tdo, a);
   PSRL_CHECK_LAUNCH();
 }
 
 // Backward of attn_fwd_sm100: qkv [T, (nq + 2 nkv) * 128], o and dout
 // [T, nq * 128] (bf16), lse [nq, T].  Returns dqkv [T, (nq + 2 nkv) * 128] bf16.
 at::Tensor attn_bwd_sm100(at::Tensor qkv, at::Tensor o, at::Tensor dout, at::Tensor lse, at::Tensor cu_seqlens,
-                          int64_t max_seqlen, int64_t nq, int64_t nkv, double scale, at::Tensor err) {
+                          int64_t max_seqlen, int64_t nq, int64_t nkv, double scale, at::Tensor err, int64_t window,
+                          int64_t sinks) {
   CHECK_CUDA_TENSOR(qkv);
   TORCH_CHECK(qkv.dim() == 2 && qkv.size(1) == (nq + 2 * nkv) * D && nq % nkv == 0, "qkv layout");
   at::cuda::CUDAGuard g(qkv.device());
@@ -1134,7 +1245,7 @@ at::Tensor attn_bwd_sm100(at::Tensor qkv, at::Tensor o, at::Tensor dout, at::Ten
   if (qkv.size(0) == 0 || cu_seqlens.numel() < 2 || max_seqlen <= 0) return dqkv.zero_();
   const int kc = (int)(nq * D), vc = (int)((nq + nkv) * D);
   bwd_launch(qkv, qkv, o, dout, lse, cu_seqlens, cu_seqlens, max_seqlen, max_seqlen, nq, nkv, 0, kc, vc, scale, dqkv,
-             0, dqkv, kc, vc, err);
+             0, dqkv, kc, vc, err, window, sinks);
   return dqkv;
 }
 
@@ -1142,7 +1253,7 @@ at::Tensor attn_bwd_sm100(at::Tensor qkv, at::Tensor o, at::Tensor dout, at::Ten
 // (bf16; key rows that no query sees get zero gradients).
 std::vector<at::Tensor> attn_bwd_sm100_kv(at::Tensor q, at::Tensor kv, at::Tensor o, at::Tensor dout, at::Tensor lse,
                                           at::Tensor cu_q, at::Tensor cu_k, int64_t max_q, int64_t max_k, int64_t nq,
-                                          int64_t nkv, double scale, at::Tensor err) {
+                                          int64_t nkv, double scale, at::Tensor err, int64_t window, int64_t sinks) {
   CHECK_CUDA_TENSOR(q);
   TORCH_CHECK(q.dim() == 2 && q.size(1) >= nq * D && kv.dim() == 2 && kv.size(1) == 2 * nkv * D && nq % nkv == 0,
               "q [Tq, nq * 128], kv [Tk, 2 nkv * 128]");
@@ -1151,7 +1262,7 @@ std::vector<at::Tensor> attn_bwd_sm100_kv(at::Tensor q, at::Tensor kv, at::Tenso
   auto dkv = at::zeros({kv.size(0), 2 * nkv * D}, q.options());
   if (q.size(0) == 0 || cu_q.numel() < 2 || max_q <= 0) return {dq.zero_(), dkv};
   bwd_launch(q, kv, o, dout, lse, cu_q, cu_k, max_q, max_k, nq, nkv, 0, 0, (int)(nkv * D), scale, dq, 0, dkv, 0,
-             (int)(nkv * D), err);
+             (int)(nkv * D), err, window, sinks);
   return {dq, dkv};
 }
 

@@ -19,12 +19,12 @@ from ._ext import ext
 
 
 # --------------------------------------------------------------- references
-def varlen_attention_ref(q, k, v, cu_seqlens, scale):
+def varlen_attention_ref(q, k, v, cu_seqlens, scale, window=None, sinks=0):
     """q [T, nq, d], k/v [T, nkv, d]; causal per sequence; fp32 math."""
     T, nq, d = q.shape
     nkv = k.shape[1]
     g = nq // nkv
-    out = torch.empty(T, nq, d, dtype=q.dtype, device=q.device)
+    out = torch.zeros(T, nq, d, dtype=q.dtype, device=q.device)
     cu = cu_seqlens.tolist()
     for i in range(len(cu) - 1):
         s, e = cu[i], cu[i + 1]
@@ -35,8 +35,8 @@ def varlen_attention_ref(q, k, v, cu_seqlens, scale):
         vs = v[s:e].float().transpose(0, 1).repeat_interleave(g, 0)
         att = (qs @ ks.transpose(1, 2)) * scale
         L = e - s
-        mask = torch.ones(L, L, dtype=torch.bool, device=q.device).triu(1)
-        att = att.masked_fill(mask, float("-inf")).softmax(-1)
+        pos = torch.arange(L, device=q.device)
+        att = att.masked_fill(~window_mask(pos[:, None], pos[None], window, sinks), float("-inf")).softmax(-1)
         out[s:e] = (att @ vs).transpose(0, 1).to(q.dtype)
     return out
 
@@ -94,7 +94,7 @@ def paged_attention_ref(q, k_cache, v_cache, cu_q, kv_lens, block_table, scale, 
     T, nq, d = q.shape
     nkv = k_cache.shape[1]
     g = nq // nkv
-    out = torch.empty_like(q)
+    out = torch.zeros_like(q)
     cu = cu_q.tolist()
     lens = kv_lens.tolist()
     for i in range(len(cu) - 1):
@@ -119,56 +119,61 @@ def paged_attention_ref(q, k_cache, v_cache, cu_q, kv_lens, block_table, scale, 
 # ----------------------------------------------------------------- autograd
 class _VarlenAttnFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, cu_seqlens, max_seqlen, nq, nkv, d, scale):
+    def forward(ctx, qkv, cu_seqlens, max_seqlen, nq, nkv, d, scale, window, sinks):
         T = qkv.shape[0]
-        o, lse = varlen_attention_fwd(qkv, cu_seqlens, max_seqlen, nq, nkv, scale, want_lse=True)
+        o, lse = varlen_attention_fwd(qkv, cu_seqlens, max_seqlen, nq, nkv, scale, True, window, sinks)
         o = o.view(T, nq, d)
         ctx.save_for_backward(qkv, o, lse, cu_seqlens)
-        ctx.cfg = (max_seqlen, nq, nkv, d, scale)
+        ctx.cfg = (max_seqlen, nq, nkv, d, scale, window, sinks)
         return o.view(T, nq * d)
 
     @staticmethod
     def backward(ctx, do):
         from .gemm import _err
         qkv, o, lse, cu = ctx.saved_tensors
-        max_seqlen, nq, nkv, d, scale = ctx.cfg
+        max_seqlen, nq, nkv, d, scale, window, sinks = ctx.cfg
         if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
             qkv = qkv.contiguous()
         # tcgen05 backward (csrc/attn_sm100.cu): dK/dV per key tile and dQ per
         # query tile, written straight into one [T, (nq + 2 nkv) * d] gradient
         dqkv = ext().attn_bwd_sm100(qkv, o.reshape(qkv.shape[0], nq * d), do.contiguous(), lse, cu, max_seqlen,
-                                    nq, nkv, scale, _err(qkv.device))
-        return dqkv, None, None, None, None, None, None
+                                    nq, nkv, scale, _err(qkv.device), window, sinks)
+        return dqkv, None, None, None, None, None, None, None, None
 
 
 def varlen_attention_fwd(qkv: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int, nq: int, nkv: int,
-                         scale: float, want_lse: bool = True):
+                         scale: float, want_lse: bool = True, window: int = 0, sinks: int = 0):
     """Forward of causal varlen attention on the tcgen05 kernel
     (``csrc/attn_sm100.cu``): ``qkv`` [T, (nq + 2 nkv) * 128] bf16 ->
-    (o [T, nq * 128] bf16, lse [nq, T] fp32 natural log)."""
+    (o [T, nq * 128] bf16, lse [nq, T] fp32 natural log).  ``window`` 0: none."""
     from .gemm import _err
     if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
         qkv = qkv.contiguous()
     return ext().attn_fwd_sm100(qkv, cu_seqlens, int(max_seqlen), int(nq), int(nkv), float(scale), bool(want_lse),
-                                _err(qkv.device))
+                                _err(qkv.device), int(window), int(sinks))
 
 
 def varlen_attention(qkv: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int, nq: int, nkv: int, d: int,
-                     scale: float | None = None) -> torch.Tensor:
-    """Causal attention over a packed batch; ``qkv`` [T, (nq+2nkv)*d] -> [T, nq*d]."""
+                     scale: float | None = None, window: int | None = None, sinks: int = 0) -> torch.Tensor:
+    """Causal attention over a packed batch; ``qkv`` [T, (nq+2nkv)*d] -> [T, nq*d].
+
+    ``window``: position p of a sequence sees only its last ``window`` positions,
+    p included, and the sequence's first ``sinks``; rows of ``qkv`` behind the
+    last sequence then give zeros, and zero gradients."""
     scale = scale if scale is not None else 1.0 / math.sqrt(d)
+    win, sinks = _window_args(window, sinks)
     if qkv.is_cuda and qkv.dtype == torch.bfloat16 and d == 128:
         if not torch.is_grad_enabled() or not qkv.requires_grad:
-            return varlen_attention_fwd(qkv, cu_seqlens, max_seqlen, nq, nkv, scale, want_lse=False)[0]
-        return _VarlenAttnFn.apply(qkv, cu_seqlens, int(max_seqlen), nq, nkv, d, scale)
+            return varlen_attention_fwd(qkv, cu_seqlens, max_seqlen, nq, nkv, scale, False, win, sinks)[0]
+        return _VarlenAttnFn.apply(qkv, cu_seqlens, int(max_seqlen), nq, nkv, d, scale, win, sinks)
     T = qkv.shape[0]
     q = qkv[:, : nq * d].view(T, nq, d)
     k = qkv[:, nq * d: (nq + nkv) * d].view(T, nkv, d)
     v = qkv[:, (nq + nkv) * d:].view(T, nkv, d)
-    return _ref_autograd(q, k, v, cu_seqlens, scale).reshape(T, nq * d)
+    return _ref_autograd(q, k, v, cu_seqlens, scale, win, sinks).reshape(T, nq * d)
 
 
-def _ref_autograd(q, k, v, cu_seqlens, scale):
+def _ref_autograd(q, k, v, cu_seqlens, scale, window=0, sinks=0):
     # differentiable reference (CPU training path)
     T, nq, d = q.shape
     nkv = k.shape[1]
@@ -183,9 +188,12 @@ def _ref_autograd(q, k, v, cu_seqlens, scale):
         ks = k[s:e].transpose(0, 1).repeat_interleave(g, 0)
         vs = v[s:e].transpose(0, 1).repeat_interleave(g, 0)
         L = e - s
-        mask = torch.ones(L, L, dtype=torch.bool, device=q.device).triu(1)
+        pos = torch.arange(L, device=q.device)
+        mask = ~window_mask(pos[:, None], pos[None], window, sinks)
         att = ((qs @ ks.transpose(1, 2)) * scale).masked_fill(mask, float("-inf")).softmax(-1)
         outs.append((att @ vs).transpose(0, 1))
+    if window and cu[-1] < T:
+        outs.append(q.new_zeros(T - cu[-1], nq, d))
     return torch.cat(outs, 0) if outs else q.new_zeros(0, nq, d)
 
 
@@ -247,7 +255,7 @@ def paged_decode_attention(q, k_cache, v_cache, block_table, kv_lens, scale=None
 
 
 # ------------------------------------------- queries against separate keys
-def attention_kv_ref(q, k, v, cu_q, cu_k, scale):
+def attention_kv_ref(q, k, v, cu_q, cu_k, scale, window=None, sinks=0):
     """q [Tq, nq, d]; k / v [Tk, nkv, d]; sequence b's queries
     [cu_q[b], cu_q[b+1]) are the last of its key positions [cu_k[b], cu_k[b+1]),
     so query row p sees keys 0 .. p + Lk - Lq.  Differentiable, fp32 math."""
@@ -264,7 +272,7 @@ def attention_kv_ref(q, k, v, cu_q, cu_k, scale):
         kk = k[ks:ke].float().transpose(0, 1).repeat_interleave(g, 0)
         vv = v[ks:ke].float().transpose(0, 1).repeat_interleave(g, 0)
         rows = torch.arange(Lq, device=q.device)[:, None] + (Lk - Lq)
-        mask = torch.arange(Lk, device=q.device)[None, :] > rows
+        mask = ~window_mask(rows, torch.arange(Lk, device=q.device)[None, :], window, sinks)
         att = ((qq @ kk.transpose(1, 2)) * scale).masked_fill(mask, float("-inf")).softmax(-1)
         outs.append((att @ vv).transpose(0, 1).to(q.dtype))
     return torch.cat(outs, 0) if outs else q.new_zeros(0, nq, d)
@@ -275,37 +283,40 @@ class _AttnKVFn(torch.autograd.Function):
     (``attn_fwd_sm100_kv`` / ``attn_bwd_sm100_kv``)."""
 
     @staticmethod
-    def forward(ctx, q, kv, cu_q, cu_k, max_q, max_k, nq, nkv, scale):
+    def forward(ctx, q, kv, cu_q, cu_k, max_q, max_k, nq, nkv, scale, window, sinks):
         from .gemm import _err
         o, lse = ext().attn_fwd_sm100_kv(q, kv, cu_q, cu_k, int(max_q), int(nq), int(nkv), float(scale), True,
-                                         _err(q.device))
+                                         _err(q.device), window, sinks)
         ctx.save_for_backward(q, kv, o, lse, cu_q, cu_k)
-        ctx.cfg = (max_q, max_k, nq, nkv, scale)
+        ctx.cfg = (max_q, max_k, nq, nkv, scale, window, sinks)
         return o
 
     @staticmethod
     def backward(ctx, do):
         from .gemm import _err
         q, kv, o, lse, cu_q, cu_k = ctx.saved_tensors
-        max_q, max_k, nq, nkv, scale = ctx.cfg
+        max_q, max_k, nq, nkv, scale, window, sinks = ctx.cfg
         dq, dkv = ext().attn_bwd_sm100_kv(q, kv, o, do.contiguous(), lse, cu_q, cu_k, int(max_q), int(max_k),
-                                          int(nq), int(nkv), float(scale), _err(q.device))
-        return dq, dkv, None, None, None, None, None, None, None
+                                          int(nq), int(nkv), float(scale), _err(q.device), window, sinks)
+        return dq, dkv, None, None, None, None, None, None, None, None, None
 
 
 def attention_kv(q: torch.Tensor, kv: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor, max_q: int, max_k: int,
-                 nq: int, nkv: int, d: int, scale: float | None = None) -> torch.Tensor:
+                 nq: int, nkv: int, d: int, scale: float | None = None, window: int | None = None,
+                 sinks: int = 0) -> torch.Tensor:
     """Causal attention of queries ``q`` [Tq, nq * d] against keys / values
     ``kv`` [Tk, 2 nkv * d] (k heads, then v heads) where each sequence's queries
     are the last ``Lq`` of its ``Lk >= Lq`` key positions; returns [Tq, nq * d].
     Context-parallel attention runs a rank's query chunks through this against
-    the gathered key prefix."""
+    the gathered key prefix.  ``window`` / ``sinks`` as in :func:`varlen_attention`."""
     scale = scale if scale is not None else 1.0 / math.sqrt(d)
+    win, sinks = _window_args(window, sinks)
     if q.is_cuda and q.dtype == torch.bfloat16 and d == 128:
         if q.stride(1) != 1 or q.stride(0) % 8 or q.data_ptr() % 16:
             q = q.contiguous()
-        return _AttnKVFn.apply(q, kv.contiguous(), cu_q, cu_k, int(max_q), int(max_k), nq, nkv, scale)
+        return _AttnKVFn.apply(q, kv.contiguous(), cu_q, cu_k, int(max_q), int(max_k), nq, nkv, scale, win,
+                              sinks)
     Tq, Tk = q.shape[0], kv.shape[0]
     o = attention_kv_ref(q.reshape(Tq, -1)[:, : nq * d].reshape(Tq, nq, d), kv[:, : nkv * d].reshape(Tk, nkv, d),
-                         kv[:, nkv * d:].reshape(Tk, nkv, d), cu_q, cu_k, scale)
+                         kv[:, nkv * d:].reshape(Tk, nkv, d), cu_q, cu_k, scale, win, sinks)
     return o.reshape(Tq, nq * d)

@@ -69,3 +69,41 @@ def attention64(q, k, v, window=None, sinks=0, scale=None):
         o[:, h] = p @ v[:, h // g]
         a[:, h] = p @ v[:, h // g].abs()
     return o, a
+
+
+def train64(q, k, v, do, window=None, sinks=0):
+    """Gradients of one sequence's attention in 64 bits with the bounds of a kernel that keeps sums in fp32 and
+    rounds the output, P and dS to bf16 (half a step: 2^-8 of the value): {name: (value, bound)}.  q, do [n, nq, D]
+    are the last n positions of k, v [L, nkv, D]."""
+    u = 2.0 ** -8
+    tiny = 2.0 ** -14                                # fp32 scores and exponentials of |score| < 2^7
+    n, nq, _ = q.shape
+    L, nkv, _ = k.shape
+    g, scale = nq // nkv, 1 / math.sqrt(D)
+    q, k, v, do = (x.double() for x in (q, k, v, do))
+    i = torch.arange(L - n, L, device=q.device)[:, None]
+    j = torch.arange(L, device=q.device)[None, :]
+    ok = j <= i
+    if window:
+        ok = ok & ((i - j < window) | (j < sinks))
+    out = {m: (torch.zeros_like(x), torch.zeros_like(x)) for m, x in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+    for h in range(nq):
+        hk = h // g
+        p = (q[:, h] @ k[:, hk].t() * scale).masked_fill(~ok, -math.inf).softmax(-1)
+        o = p @ v[:, hk]
+        eo = u * o.abs() + (u + tiny) * (p @ v[:, hk].abs())
+        dp = do[:, h] @ v[:, hk].t()
+        dd = (o * do[:, h]).sum(-1, keepdim=True)
+        ed = (eo * do[:, h].abs()).sum(-1, keepdim=True)
+        ds = p * (dp - dd)
+        es = u * ds.abs() + p * (ed + tiny * (dp.abs() + dd.abs()))
+        out["o"][0][:, h], out["o"][1][:, h] = o, eo
+        out["dq"][0][:, h] = ds @ k[:, hk] * scale
+        out["dq"][1][:, h] = es @ k[:, hk].abs() * scale
+        out["dk"][0][:, hk] += ds.t() @ q[:, h] * scale
+        out["dk"][1][:, hk] += es.t() @ q[:, h].abs() * scale
+        out["dv"][0][:, hk] += p.t() @ do[:, h]
+        out["dv"][1][:, hk] += (u + tiny) * (p.t() @ do[:, h].abs())
+    for m in ("dq", "dk", "dv"):
+        out[m][1].add_(u * out[m][0].abs())          # the gradient's own rounding
+    return out
