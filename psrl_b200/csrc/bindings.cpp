@@ -34,6 +34,10 @@ at::Tensor attn_decode(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at:
 at::Tensor attn_decode_fp8(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, at::Tensor k_scale, at::Tensor v_scale,
                            at::Tensor block_table, at::Tensor kv_lens, double scale, int64_t window, int64_t sinks,
                            at::Tensor err);
+at::Tensor attn_paged_chunk(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache, c10::optional<at::Tensor> k_scale,
+                            c10::optional<at::Tensor> v_scale, at::Tensor cu_q, at::Tensor kv_lens,
+                            at::Tensor block_table, int64_t max_q_len, double scale, int64_t window, int64_t sinks,
+                            at::Tensor err);
 at::Tensor rope_quant_kv(at::Tensor qkv, at::Tensor positions, at::Tensor cos_t, at::Tensor sin_t, int64_t nq,
                          int64_t nkv, int64_t d, at::Tensor k_cache, at::Tensor v_cache, at::Tensor k_scale,
                          at::Tensor v_scale, at::Tensor slots);
@@ -112,6 +116,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("block_table"), pybind11::arg("kv_lens"), pybind11::arg("scale"), pybind11::arg("splits"), pybind11::arg("scratch"),
         pybind11::arg("stages") = 0, pybind11::arg("window") = 0, pybind11::arg("sinks") = 0);
   m.def("attn_decode_fp8", &psrl::attn_decode_fp8);
+  m.def("attn_paged_chunk", &psrl::attn_paged_chunk);
   m.def("rope_quant_kv", &psrl::rope_quant_kv);
   m.def("read_kv_cache", &psrl::read_kv_cache, py::arg("cache"), py::arg("scale"), py::arg("blocks"), py::arg("out"),
         py::arg("out_blocks") = py::none());

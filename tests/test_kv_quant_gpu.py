@@ -243,3 +243,140 @@ def test_refusals():
                           torch.zeros(2, dtype=torch.int32, device=dev), 4, 2, D, 1e6, k, v, ks, vs,
                           torch.zeros(3, dtype=torch.int32, device=dev))
     assert call(q[:0], k, v, table[:0], lens[:0], k_scale=ks, v_scale=vs).shape == (0, 4, D)
+
+
+# -------------------------------------------------------------------- chunk
+def _check_chunk(new, lens, nq, nkv, bs, bits, window=None, sinks=0, seed=0, pad=0, tail=0, max_q=None):
+    from psrl_b200.ops.gemm import check_errors
+    gen = torch.Generator().manual_seed(seed)
+    k, v, ks, vs, table, kd, vd = pages(gen, lens, nkv, bs, bits)
+    T = sum(new) + tail
+    q = torch.randn(T, nq * (D + pad), generator=gen).to(torch.bfloat16).view(T, nq, D + pad)[:, :, :D]
+    if tail:
+        q = q.clone()
+        q[-tail:] = math.nan
+    dk, dv, dks, dvs, dt = _cuda(k, v, ks, vs, table)
+    dq = torch.empty(T, nq, D + pad, dtype=torch.bfloat16, device=dev)[:, :, :D]
+    dq.copy_(q)
+    cu = torch.tensor([0] + new).cumsum(0).to(torch.int32).to(dev)
+    o = ops.paged_prefill_attention(dq, dk, dv, cu, torch.tensor(lens, dtype=torch.int32, device=dev), dt,
+                                    max_q or max(new), k_scale=dks, v_scale=dvs, window=window, sinks=sinks).cpu().double()
+    check_errors()
+    at = 0
+    for i, n in enumerate(new):
+        m = min(n, lens[i])                          # queries before position 0 see nothing: zeros
+        ref, mag = attention64(q[at + n - m: at + n], kd[i], vd[i], window, sinks)
+        # P is bf16 whatever the cache's type
+        worst = ((o[at + n - m: at + n] - ref).abs() / (_decode_bound(ref, mag, 16) + 1e-30)).max() if m else 0
+        assert worst <= 1, (i, n, lens[i], float(worst))
+        assert (o[at: at + n - m] == 0).all()
+        at += n
+    assert (o[at:] == 0).all()
+
+
+NEW = [1, 5, 16, 17, 64, 130, 300, 3, 0, 2, 1]
+CTX = [1, 200, 16, 129, 1000, 130, 511, 3, 40, 1, 0]
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("nq,nkv", [(16, 2), (28, 4), (8, 8), (32, 2), (3, 1), (64, 1)])
+def test_chunk_heads(nq, nkv, bits):
+    win = dict() if bits == 8 else dict(window=150, sinks=5)
+    _check_chunk(NEW, CTX, nq, nkv, 64, bits, seed=nq, pad=8 if nq == 28 else 0, tail=9, **win)
+
+
+@pytest.mark.parametrize("bs", [16, 32, 128, 512])
+def test_chunk_pages(bs):
+    _check_chunk(NEW, CTX, 8, 2, bs, 8, seed=bs)
+    _check_chunk(NEW, CTX, 8, 2, bs, 16, 100, 4, seed=bs)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (64, 0), (128, 130), (200, 4), (5000, 0)])
+def test_chunk_window(bits, window, sinks):
+    _check_chunk(NEW, CTX, 8, 2, 64, bits, window, sinks, seed=window)
+
+
+def test_chunk_split_and_whole():
+    _check_chunk([5], [3000], 16, 2, 64, 8, seed=1)                      # few tokens, long context: keys are split
+    _check_chunk([5, 1, 33], [3000, 2, 900], 8, 8, 64, 8, seed=2)
+    _check_chunk([5], [3000], 16, 2, 64, 8, 300, 70, seed=3)
+    _check_chunk([1500], [1500], 32, 8, 64, 8, seed=4, max_q=4000)       # many blocks: whole; max_q may be an upper bound
+
+
+def test_chunk_extreme_exponents_and_nan():
+    gen = torch.Generator().manual_seed(5)
+    nq, nkv, bs, L, n = 8, 2, 64, 300, 40
+    k, v, ks, vs, table, kd, vd = pages(gen, [L], nkv, bs, 8)
+    p = torch.arange(L)
+    at = table[0, :5].long()[p // bs]
+    size = torch.exp2(torch.randint(-60, 110, (L, nkv, 1), generator=gen).double())
+    size[::7] = 0
+    codes, byte = quantise_ref((torch.randn(L, nkv, D, generator=gen).double() * size).to(torch.bfloat16))
+    v.view(torch.uint8)[at, :, p % bs] = codes.view(torch.uint8)
+    vs[at, :, p % bs] = byte
+    vd = dequantise_ref(codes, byte, torch.float64)
+    q = torch.randn(n, nq, D, generator=gen).to(torch.bfloat16)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+    call = lambda **w: ops.paged_prefill_attention(  # noqa: E731
+        *_cuda(q, k, v), cu, torch.tensor([L], dtype=torch.int32, device=dev), table.to(dev), n,
+        k_scale=ks.to(dev), v_scale=vs.to(dev), **w).cpu().double()
+    ref, mag = attention64(q, kd[0], vd)
+    assert ((call() - ref).abs() <= _decode_bound(ref, mag, 16)).all()
+    # a NaN value vector at position 280 (kv head 1): only the rows that see it
+    vs[at[280], 1, 280 % bs] = 255
+    o = call()
+    assert torch.isnan(o[280 - (L - n):, 4:]).all()
+    assert torch.isfinite(o[: 280 - (L - n)]).all() and torch.isfinite(o[:, :4]).all()
+    o = call(window=10)
+    first = 280 - (L - n)
+    assert torch.isnan(o[first: first + 10, 4:]).all() and torch.isfinite(o[first + 10:]).all()
+
+
+def test_chunk_graph():
+    gen = torch.Generator().manual_seed(6)
+    nq, nkv, lens, new = 16, 2, [700, 90], [30, 64]
+    k, v, ks, vs, table, kd, vd = pages(gen, lens, nkv, 64, 8)
+    q = torch.randn(sum(new), nq, D, generator=gen).to(torch.bfloat16)
+    dk, dv, dks, dvs, dt, dq = _cuda(k, v, ks, vs, table, q)
+    cu = torch.tensor([0, 30, 94], dtype=torch.int32, device=dev)
+    dl = torch.tensor(lens, dtype=torch.int32, device=dev)
+    run = lambda: ops.paged_prefill_attention(dq, dk, dv, cu, dl, dt, 64, k_scale=dks, v_scale=dvs)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = run()
+    for new_lens in ([700, 90], [31, 64], [256, 65]):
+        dl.copy_(torch.tensor(new_lens, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, run())
+        for i, (a, b) in enumerate(((0, 30), (30, 94))):
+            ref, mag = attention64(q[a:b], kd[i][:new_lens[i]], vd[i][:new_lens[i]])
+            assert ((o[a:b].cpu().double() - ref).abs() <= _decode_bound(ref, mag, 16)).all()
+
+
+def test_chunk_refusals():
+    gen = torch.Generator().manual_seed(3)
+    k, v, ks, vs, table = _cuda(*pages(gen, [9], 2, 16, 8)[:5])
+    q = torch.randn(4, 4, D, device=dev).to(torch.bfloat16)
+    cu = torch.tensor([0, 4], dtype=torch.int32, device=dev)
+    lens = torch.tensor([9], dtype=torch.int32, device=dev)
+    call = ops.paged_prefill_attention
+    with pytest.raises(ValueError, match="both k_scale"):
+        call(q, k, v, cu, lens, table, 4, k_scale=ks)
+    with pytest.raises(RuntimeError, match="cu_q"):
+        call(q, k, v, cu.long(), lens, table, 4, k_scale=ks, v_scale=vs)
+    with pytest.raises(RuntimeError, match="block_table"):
+        call(q, k, v, cu, lens, table[:, 0], 4, k_scale=ks, v_scale=vs)
+    with pytest.raises(RuntimeError, match="kv_lens"):
+        call(q, k, v, cu, lens.cpu(), table, 4, k_scale=ks, v_scale=vs)
+    with pytest.raises(RuntimeError, match="multiple"):
+        call(q[:, :3], k, v, cu, lens, table, 4, k_scale=ks, v_scale=vs)
+    with pytest.raises(ValueError, match="window"):
+        call(q, k, v, cu, lens, table, 4, k_scale=ks, v_scale=vs, window=0)
+    assert call(q[:0], k, v, cu[:1] * 0, lens[:0], table[:0], 0, k_scale=ks, v_scale=vs).shape == (0, 4, D)
