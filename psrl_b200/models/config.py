@@ -39,7 +39,9 @@ class ModelArgs:
     shared_expert_intermediate_size: int = 0   # Qwen2-MoE: always-on expert with a sigmoid gate
     hidden_act: str = "silu"            # silu (SwiGLU) | gelu_tanh (GeGLU, Gemma)
     embed_scale: float = 0.0            # Gemma: embeddings multiplied by sqrt(hidden)
-    sliding_window: int | None = None   # Mistral: attention window (must cover the whole context)
+    sliding_window: int | None = None   # Mistral: a position sees the last sliding_window positions
+    window_from_layer: int = 0          # Qwen2's max_window_layers: layers before it attend to the whole context
+    attention_sinks: int = 0            # first tokens of a sequence that stay visible to a windowed layer
     extra: dict = field(default_factory=dict)
 
     @property
@@ -67,12 +69,11 @@ class ModelArgs:
         return (float(self.rope_theta),) + tuple(sorted((k, v) for k, v in self.rope_scaling.items()
                                                         if not isinstance(v, (list, dict))))
 
-    def check_context(self, length: int) -> None:
-        """Sliding-window attention is implemented only as full attention, which
-        is exact while the window covers the whole context."""
-        if self.sliding_window is not None and length > self.sliding_window:
-            raise NotImplementedError(f"context of {length} tokens exceeds the {self.sliding_window}-token "
-                                      "sliding window; windowed attention is not implemented")
+    def layer_window(self, layer: int) -> dict:
+        """The attention ops' ``window`` / ``sinks`` arguments of a layer."""
+        if self.sliding_window is None or layer < self.window_from_layer:
+            return {}
+        return {"window": int(self.sliding_window), "sinks": int(self.attention_sinks)}
 
     def num_params(self) -> int:
         h, L = self.hidden_size, self.num_layers

@@ -10,8 +10,7 @@ families register with :func:`register_family`.
 
 Supported ``model_type`` values: ``qwen2``, ``qwen3``, ``qwen3_moe``,
 ``qwen2_moe`` (shared expert with a sigmoid gate), ``llama`` (incl. Llama-3
-RoPE scaling), ``mistral`` (sliding window only where it spans the whole
-context), ``mixtral``, ``olmoe`` (q/k RMSNorm over the full projection),
+RoPE scaling), ``mistral`` (sliding-window attention), ``mixtral``, ``olmoe`` (q/k RMSNorm over the full projection),
 ``phi3`` (fused ``qkv_proj`` / ``gate_up_proj`` in the checkpoint) and
 ``gemma`` (GeGLU, embeddings scaled by sqrt(hidden), RMSNorm weights stored as
 ``w - 1``).
@@ -115,6 +114,13 @@ def args_from_hf_config(cfg: dict) -> ModelArgs:
     window = cfg.get("sliding_window")
     if not cfg.get("use_sliding_window", mt in ("mistral",)) or not window:
         window = None
+    # the layers that have the window: Qwen2's from max_window_layers on, or listed one by one
+    first = int(cfg.get("max_window_layers") or 0) if window and mt in ("qwen2", "qwen2_moe") else 0
+    kinds = cfg.get("layer_types")
+    if window and kinds:
+        first = next((i for i, k in enumerate(kinds) if k == "sliding_attention"), len(kinds))
+        if any(k != "sliding_attention" for k in kinds[first:]):
+            raise NotImplementedError("layers with full attention above layers with a sliding window")
     n_exp = int(cfg.get("num_experts", cfg.get("num_local_experts", 0)) or 0) if f.moe else 0
     a = ModelArgs(
         arch=mt,
@@ -141,6 +147,7 @@ def args_from_hf_config(cfg: dict) -> ModelArgs:
         hidden_act=act,
         embed_scale=float(cfg["hidden_size"]) ** 0.5 if mt == "gemma" else 0.0,
         sliding_window=window,
+        window_from_layer=first,
         extra={"hf_tokens": {k: cfg[k] for k in _TOKEN_KEYS if cfg.get(k) is not None}},
     )
     return a
@@ -173,6 +180,8 @@ def hf_config_from_args(a: ModelArgs) -> dict:
         d["sliding_window"] = a.sliding_window
         if f.model_type in ("qwen2", "qwen2_moe"):
             d["use_sliding_window"] = a.sliding_window is not None
+            if a.sliding_window is not None:
+                d["max_window_layers"] = a.window_from_layer
     if a.is_moe:
         key = "num_local_experts" if f.model_type == "mixtral" else "num_experts"
         d.update({key: a.num_experts, "num_experts_per_tok": a.num_experts_per_tok,

@@ -39,9 +39,10 @@ from .config import ModelArgs
 
 
 class Attention(nn.Module):
-    def __init__(self, a: ModelArgs):
+    def __init__(self, a: ModelArgs, layer: int = 0):
         super().__init__()
         self.a = a
+        self.window = a.layer_window(layer)
         self.qkv = nn.Linear(a.hidden_size, a.qkv_size, bias=a.qkv_bias)
         self.o = nn.Linear(a.q_size, a.hidden_size, bias=False)
         if a.qk_norm:
@@ -69,13 +70,14 @@ class Attention(nn.Module):
         if isinstance(cu_seqlens, CPPlan):
             # context parallel: this rank's query chunks over the gathered keys
             o = cp_attention(qkv[:, : a.q_size], qkv[:, a.q_size:], cu_seqlens, a.num_heads, a.num_kv_heads,
-                             a.head_dim)
+                             a.head_dim, **self.window)
         elif isinstance(cu_seqlens, UlyssesPlan):
             # Ulysses: all-to-all to head-parallel attention over the whole micro-batch and back
             o = ulysses_attention(qkv[:, : a.q_size], qkv[:, a.q_size:], cu_seqlens, a.num_heads,
-                                  a.num_kv_heads, a.head_dim)
+                                  a.num_kv_heads, a.head_dim, **self.window)
         else:
-            o = ops.varlen_attention(qkv, cu_seqlens, max_seqlen, a.num_heads, a.num_kv_heads, a.head_dim)
+            o = ops.varlen_attention(qkv, cu_seqlens, max_seqlen, a.num_heads, a.num_kv_heads, a.head_dim,
+                                     **self.window)
         return linear(o, self.o.weight)
 
 
@@ -161,12 +163,12 @@ class MoE(nn.Module):
 
 
 class DecoderLayer(nn.Module):
-    def __init__(self, a: ModelArgs):
+    def __init__(self, a: ModelArgs, layer: int = 0):
         super().__init__()
         self.a = a
         self.ln1 = nn.Parameter(torch.ones(a.hidden_size))
         self.ln2 = nn.Parameter(torch.ones(a.hidden_size))
-        self.attn = Attention(a)
+        self.attn = Attention(a, layer)
         self.mlp = MoE(a) if a.is_moe else MLP(a)
 
     def forward(self, x, resid, positions, cu_seqlens, max_seqlen):
@@ -185,7 +187,7 @@ class QwenModel(nn.Module):
         super().__init__()
         self.args = a
         self.embed = nn.Embedding(a.vocab_size, a.hidden_size)
-        self.layers = nn.ModuleList([DecoderLayer(a) for _ in range(a.num_layers)])
+        self.layers = nn.ModuleList([DecoderLayer(a, i) for i in range(a.num_layers)])
         self.norm = nn.Parameter(torch.ones(a.hidden_size))
         if a.value_head:
             self.value = nn.Linear(a.hidden_size, 1, bias=True)
@@ -215,8 +217,6 @@ class QwenModel(nn.Module):
     # --------------------------------------------------------------- forward
     def hidden_states(self, input_ids, positions, cu_seqlens, max_seqlen):
         a = self.args
-        if a.sliding_window is not None and not isinstance(cu_seqlens, (CPPlan, UlyssesPlan)):
-            a.check_context(int(max_seqlen))
         x = self.embed(input_ids)
         if a.embed_scale:
             x = x * torch.tensor(a.embed_scale, dtype=x.dtype)

@@ -88,9 +88,6 @@ def _paged_args(q, k_cache, v_cache, k_scale, v_scale):
 def paged_attention_ref(q, k_cache, v_cache, cu_q, kv_lens, block_table, scale, k_scale=None, v_scale=None,
                         window=None, sinks=0):
     """Queries are the last q_len positions of each context (causal)."""
-    if k_scale is not None:
-        from .kv_quant import dequantise_ref
-        k_cache, v_cache = dequantise_ref(k_cache, k_scale), dequantise_ref(v_cache, v_scale)
     T, nq, d = q.shape
     nkv = k_cache.shape[1]
     g = nq // nkv
@@ -102,7 +99,13 @@ def paged_attention_ref(q, k_cache, v_cache, cu_q, kv_lens, block_table, scale, 
         if e <= s:
             continue
         L = lens[i]
-        k, v = gather_paged_kv(k_cache, v_cache, block_table[i], L)
+        if k_scale is None:
+            k, v = gather_paged_kv(k_cache, v_cache, block_table[i], L)
+        else:
+            from .kv_quant import read_kv_cache
+            ids = block_table[i, : -(-L // k_cache.shape[2])].long()
+            k, v = (read_kv_cache(c, e, ids).transpose(1, 2).reshape(-1, nkv, d)[:L]
+                    for c, e in ((k_cache, k_scale), (v_cache, v_scale)))
         qs = q[s:e].float().transpose(0, 1)
         ks = k.float().transpose(0, 1).repeat_interleave(g, 0)
         vs = v.float().transpose(0, 1).repeat_interleave(g, 0)

@@ -136,12 +136,13 @@ class _AllGatherRows(torch.autograd.Function):
 
 
 def cp_attention(q: torch.Tensor, kv: torch.Tensor, plan: CPPlan, nq: int, nkv: int, d: int,
-                 scale: float | None = None) -> torch.Tensor:
+                 scale: float | None = None, window: int | None = None, sinks: int = 0) -> torch.Tensor:
     """Attention of this rank's queries ``q`` [T_loc, nq d] over the whole
     sequences, given this rank's keys / values ``kv`` [T_loc, 2 nkv d]."""
     full = _AllGatherRows.apply(kv, plan.group)[plan.perm]          # sequence order
     kv_pref = full.index_select(0, plan.kv_idx)                       # each chunk's key prefix
-    return attention_kv(q, kv_pref, plan.cu_q, plan.cu_k, plan.max_q, plan.max_k, nq, nkv, d, scale)
+    return attention_kv(q, kv_pref, plan.cu_q, plan.cu_k, plan.max_q, plan.max_k, nq, nkv, d, scale,
+                        window, sinks)
 
 
 def gather_tokens(x: torch.Tensor, plan: CPPlan) -> torch.Tensor:

@@ -113,6 +113,7 @@ class TPAttention(nn.Module):
                           a.q_size + torch.arange(r * kn, (r + 1) * kn),
                           a.q_size + a.kv_size + torch.arange(r * kn, (r + 1) * kn)])
         w = full.qkv.weight.data
+        self.window = full.window
         self.qkv_weight = nn.Parameter(w.index_select(0, rows.to(w.device)).clone())
         self.qkv_bias = None
         if full.qkv.bias is not None:
@@ -138,7 +139,8 @@ class TPAttention(nn.Module):
             k = ops.head_rms_norm(k.reshape(T, la.num_kv_heads, la.head_dim), self.k_norm, la.rms_eps).reshape(T, -1)
             qkv = torch.cat([q, k, v], dim=-1)
         qkv = ops.rope_qkv(qkv.contiguous(), positions, la.num_heads, la.num_kv_heads, la.head_dim, la.rope_spec)
-        o = ops.varlen_attention(qkv, cu_seqlens, max_seqlen, la.num_heads, la.num_kv_heads, la.head_dim)
+        o = ops.varlen_attention(qkv, cu_seqlens, max_seqlen, la.num_heads, la.num_kv_heads, la.head_dim,
+                                 **self.window)
         if self.tp.fused_fits(o, self.a.hidden_size) and T == o.shape[0]:
             from .tp_fused import row_parallel
             return row_parallel(o, self.o_weight, self.tp.fused)

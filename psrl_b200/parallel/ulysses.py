@@ -88,7 +88,7 @@ class _HeadsToRows(torch.autograd.Function):
 
 
 def ulysses_attention(q: torch.Tensor, kv: torch.Tensor, plan: UlyssesPlan, nq: int, nkv: int,
-                      d: int) -> torch.Tensor:
+                      d: int, window: int | None = None, sinks: int = 0) -> torch.Tensor:
     """q [T_loc, nq d] and kv [T_loc, 2 nkv d] (k heads, then v heads) of this
     rank's rows -> attention output [T_loc, nq d] of the same rows."""
     P = plan.world
@@ -100,7 +100,7 @@ def ulysses_attention(q: torch.Tensor, kv: torch.Tensor, plan: UlyssesPlan, nq: 
     x = torch.cat([q.reshape(t, P, qh * d), kv[:, : nkv * d].reshape(t, P, kh * d),
                    kv[:, nkv * d:].reshape(t, P, kh * d)], dim=-1).reshape(t, -1)
     y = _RowsToHeads.apply(x, plan.group, P)                                  # [T_pad, (qh + 2 kh) d]
-    o = ops.varlen_attention(y[: plan.n_real].contiguous(), plan.cu, plan.max_q, qh, kh, d)
+    o = ops.varlen_attention(y[: plan.n_real].contiguous(), plan.cu, plan.max_q, qh, kh, d, window=window, sinks=sinks)
     if plan.t_pad > plan.n_real:                                              # padding rows: zero output
         o = torch.cat([o, o.new_zeros(plan.t_pad - plan.n_real, o.shape[1])])
     return _HeadsToRows.apply(o, plan.group, P)

@@ -37,7 +37,7 @@ from ..ops.linear import decode_gate_up_swiglu, decode_linear, gate_up_swiglu
 from ..ops.linear import linear as linear_tc
 from ..utils import transfer
 from ..models.config import ModelArgs
-from .kv_cache import BlockManager, allocate_kv_tensors
+from .kv_cache import BlockManager, allocate_kv_scales, allocate_kv_tensors
 
 
 @dataclass
@@ -168,7 +168,7 @@ class RolloutEngine:
                  kv_cache_gb: float | None = None, num_blocks: int | None = None, enable_prefix_caching: bool = True,
                  use_cuda_graph: bool = True, keep_kv_on_update: bool = False, version: int = 0,
                  eos_token_id: int | None = None, tp=None, memory_pool=None, decode_gemm: str = "library",
-                 kv_offload_blocks: int = 0):
+                 kv_offload_blocks: int = 0, kv_cache_dtype: str = "auto"):
         # tensor parallelism (``tp``: parallel.tp.TPGroup): this engine holds query heads,
         # KV heads and MLP columns [r/P, (r+1)/P) of every layer (weights in the same
         # layout as the TP trainer's shards) and its KV cache for its own KV heads; the
@@ -204,7 +204,6 @@ class RolloutEngine:
         self.dtype = weights.dtype
         self.max_num_seqs = int(max_num_seqs)
         self.max_model_len = int(max_model_len)
-        args.check_context(self.max_model_len)
         self.block_size = int(block_size)
         self.max_blocks_per_seq = math.ceil(self.max_model_len / self.block_size)
         self.max_num_batched_tokens = int(max_num_batched_tokens)
@@ -213,7 +212,19 @@ class RolloutEngine:
         self.version = int(version)
         self.eos_token_id = eos_token_id
         a = args
-        per_block = 2 * a.num_layers * a.num_kv_heads * self.block_size * a.head_dim * torch.finfo(self.dtype).bits // 8
+        # KV cache type: "auto" (the weights' dtype) or "fp8" (float8 codes and one
+        # exponent byte per token and kv head, ops/kv_quant.py: half the bytes a
+        # decode step reads, twice the tokens a cache holds)
+        if kv_cache_dtype not in ("auto", "fp8"):
+            raise ValueError(f"kv_cache_dtype must be 'auto' or 'fp8', not {kv_cache_dtype!r}")
+        fp8 = kv_cache_dtype == "fp8"
+        if fp8 and self.device.type == "cuda" and (a.head_dim != 128 or self.dtype != torch.bfloat16
+                                                   or self.block_size < 16 or self.block_size & (self.block_size - 1)):
+            raise ValueError("an fp8 KV cache needs bf16 weights, head_dim 128 and a block size that is a power of two "
+                             f">= 16, not {self.dtype}, {a.head_dim} and {self.block_size}")
+        self.kv_dtype = torch.float8_e4m3fn if fp8 else self.dtype
+        vec_bytes = a.head_dim + 1 if fp8 else a.head_dim * torch.finfo(self.dtype).bits // 8
+        per_block = 2 * a.num_layers * a.num_kv_heads * self.block_size * vec_bytes
         if num_blocks is None:
             gb = kv_cache_gb if kv_cache_gb is not None else 4.0
             num_blocks = max(2 * self.max_blocks_per_seq, int(gb * (1 << 30) // per_block))
@@ -237,8 +248,12 @@ class RolloutEngine:
         if memory_pool is not None:
             weights.move_to_pool(memory_pool, "weights")
         self.k_cache, self.v_cache = allocate_kv_tensors(a.num_layers, self.num_blocks, a.num_kv_heads,
-                                                         self.block_size, a.head_dim, self.dtype, self.device,
+                                                         self.block_size, a.head_dim, self.kv_dtype, self.device,
                                                          pool=memory_pool)
+        self.k_scale = self.v_scale = None
+        if fp8:
+            self.k_scale, self.v_scale = allocate_kv_scales(a.num_layers, self.num_blocks, a.num_kv_heads,
+                                                            self.block_size, self.device, pool=memory_pool)
         if int(kv_offload_blocks) > 0:
             from .kv_offload import KVOffloadStore
             self.offload = KVOffloadStore(self, int(kv_offload_blocks))
@@ -353,13 +368,15 @@ class RolloutEngine:
         peer GPU over NVLink, or host memory), so ``dst`` continues it with a
         one-token prefill instead of recomputing the context.  Both engines must
         hold the same weight version.  Returns False (and keeps the request) when
-        ``dst`` has no room."""
-        from .kv_offload import transfer_direct
+        ``dst`` has no room, or its cache's type cannot take this one's blocks (an
+        8-bit cache's go to a bf16 one on the same GPU, not the other way)."""
+        from .kv_offload import can_transfer, transfer_direct
         self._drain(self.finished_unreported)
         dst._drain(dst.finished_unreported)
         s = self.by_id.get(request_id)
         bs = self.block_size
-        if s is None or dst is self or dst.asleep or dst.version != self.version or dst.block_size != bs:
+        if s is None or dst is self or dst.asleep or dst.version != self.version or dst.block_size != bs \
+                or not can_transfer(self, dst):
             return False
         need = -(-s.num_computed // bs)
         if dst.num_unfinished() >= dst.max_num_seqs or not dst.bm.can_allocate(need + 1):
@@ -897,15 +914,24 @@ class RolloutEngine:
                 k = qkv[:, a.q_size: a.q_size + a.kv_size]
                 q.copy_(ops.rms_norm(q.contiguous(), W[pre + "attn.q_norm"], a.rms_eps)[0])
                 k.copy_(ops.rms_norm(k.contiguous(), W[pre + "attn.k_norm"], a.rms_eps)[0])
-            ops.rope_qkv_(qkv, pos, a.num_heads, a.num_kv_heads, a.head_dim, a.rope_spec,
-                          k_cache=self.k_cache[l], v_cache=self.v_cache[l], slots=slots)
-            q = qkv[:, : a.q_size].view(T, a.num_heads, a.head_dim)
-            if mode == "prefill":
-                o = ops.paged_prefill_attention(q, self.k_cache[l], self.v_cache[l], cu_q, kv_lens, block_table, max_q)
+            how = a.layer_window(l)
+            if self.k_scale is not None:
+                how.update(k_scale=self.k_scale[l], v_scale=self.v_scale[l])
+                q = ops.rope_quant_kv(qkv, pos, a.num_heads, a.num_kv_heads, a.head_dim, a.rope_spec, self.k_cache[l],
+                                      self.v_cache[l], self.k_scale[l], self.v_scale[l], slots)
             else:
+                ops.rope_qkv_(qkv, pos, a.num_heads, a.num_kv_heads, a.head_dim, a.rope_spec,
+                              k_cache=self.k_cache[l], v_cache=self.v_cache[l], slots=slots)
+                q = qkv[:, : a.q_size]
+            q = q.view(T, a.num_heads, a.head_dim)
+            if mode == "prefill":
+                o = ops.paged_prefill_attention(q, self.k_cache[l], self.v_cache[l], cu_q, kv_lens, block_table, max_q,
+                                                **how)
+            else:
+                # a windowed layer's keys are few: its own number of splits
                 o = ops.paged_decode_attention(q, self.k_cache[l], self.v_cache[l], block_table, kv_lens,
-                                               splits=splits if self.is_cuda else None,
-                                               scratch=self.decode_scratch if self.is_cuda else None)
+                                               splits=splits if self.is_cuda and "window" not in how else None,
+                                               scratch=self.decode_scratch if self.is_cuda else None, **how)
             attn = proj(o.reshape(T, a.q_size), W[pre + "attn.o.weight"])
             if self.tp is not None:
                 dist.all_reduce(attn, group=self.tp.group)

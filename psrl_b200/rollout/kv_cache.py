@@ -7,6 +7,8 @@
 * Full blocks are content-addressed by a hash chain over (parent hash, the
   block's tokens, weight version); a new request whose prompt starts with a
   cached chain reuses those blocks (multi-turn prefix reuse, K1/K2).
+* An 8-bit cache (``ops/kv_quant.py``) is float8 codes of that shape and one
+  exponent byte per (token, kv head): two more lists of tensors.
 * Blocks are reference counted; blocks whose count drops to zero stay in the
   content index and are reclaimed in LRU order when the free list is empty.
 * The weight version is part of the hash, so a weight update never serves KV
@@ -126,6 +128,9 @@ def allocate_kv_tensors(num_layers: int, num_blocks: int, nkv: int, block_size: 
     in one driver virtual-memory region per tensor under ``tag``, so the engine
     can release its physical memory while asleep and keep the addresses."""
     shape = (num_blocks, nkv, block_size, head_dim)
+    if dtype == torch.float8_e4m3fn:
+        k, v = allocate_kv_tensors(num_layers, num_blocks, nkv, block_size, head_dim, torch.uint8, device, pool, tag)
+        return [t.view(dtype) for t in k], [t.view(dtype) for t in v]
     if pool is not None:
         k = [pool.tensor(tag, shape, dtype) for _ in range(num_layers)]
         v = [pool.tensor(tag, shape, dtype) for _ in range(num_layers)]
@@ -135,3 +140,10 @@ def allocate_kv_tensors(num_layers: int, num_blocks: int, nkv: int, block_size: 
     k = [torch.zeros(*shape, dtype=dtype, device=device) for _ in range(num_layers)]
     v = [torch.zeros(*shape, dtype=dtype, device=device) for _ in range(num_layers)]
     return k, v
+
+
+def allocate_kv_scales(num_layers: int, num_blocks: int, nkv: int, block_size: int, device, pool=None, tag: str = "kv"):
+    """Exponent bytes of an 8-bit cache: two lists (K, V) of per-layer
+    [num_blocks, nkv, block_size] uint8 tensors."""
+    k, v = allocate_kv_tensors(num_layers, num_blocks, nkv, block_size, 1, torch.uint8, device, pool, tag)
+    return [t.squeeze(-1) for t in k], [t.squeeze(-1) for t in v]

@@ -7,7 +7,8 @@ blocks can be pinned so they are never evicted.  ``transfer_direct`` copies a
 request's blocks from one engine's cache into another's (a peer GPU over
 NVLink via an IPC mapping, or the same GPU) — used when the router migrates a
 partially generated request.  All moves are one ``kv_copy_blocks`` kernel over
-every layer's K and V.  Reference: ``psrl/utils/kv_cache/manager.py``.
+every layer's K and V (and one over the exponent bytes of an 8-bit cache);
+blocks of an 8-bit cache go to a bf16 one through ``ops.read_kv_cache``.  Reference: ``psrl/utils/kv_cache/manager.py``.
 """
 
 from __future__ import annotations
@@ -41,7 +42,24 @@ def copy_blocks(src_k, src_v, dst_k, dst_v, src_blocks, dst_blocks, device=None)
                                  src_k[0].shape[0], dst_k[0].shape[0])
         return
     for s, d in zip(list(src_k) + list(src_v), list(dst_k) + list(dst_v)):
+        if s.dtype == torch.float8_e4m3fn:
+            s, d = s.view(torch.uint8), d.view(torch.uint8)
         d[torch.tensor(dst_blocks)] = s[torch.tensor(src_blocks)].to(d.device)
+
+
+def _tensors(side):
+    """(K, V, K exponents, V exponents) lists of an engine or a host store."""
+    k, v = (side.k, side.v) if isinstance(side, KVOffloadStore) else (side.k_cache, side.v_cache)
+    return k, v, side.k_scale, side.v_scale
+
+
+def copy_cache(src, dst, src_blocks, dst_blocks, device) -> None:
+    """Blocks of one cache (engine or host store) into another of the same type."""
+    sk, sv, sks, svs = _tensors(src)
+    dk, dv, dks, dvs = _tensors(dst)
+    copy_blocks(sk, sv, dk, dv, src_blocks, dst_blocks, device)
+    if sks is not None:
+        copy_blocks(sks, svs, dks, dvs, src_blocks, dst_blocks, device)
 
 
 class KVOffloadStore:
@@ -50,8 +68,13 @@ class KVOffloadStore:
         a = engine.args
         shape = (capacity_blocks, a.num_kv_heads, engine.block_size, a.head_dim)
         pin = engine.device.type == "cuda"
-        self.k = [torch.zeros(shape, dtype=engine.dtype, pin_memory=pin) for _ in range(a.num_layers)]
-        self.v = [torch.zeros(shape, dtype=engine.dtype, pin_memory=pin) for _ in range(a.num_layers)]
+        fp8 = engine.k_scale is not None
+        make = lambda sh, dt: [torch.zeros(sh, dtype=dt, pin_memory=pin) for _ in range(a.num_layers)]  # noqa: E731
+        self.k, self.v = (make(shape, torch.uint8 if fp8 else engine.dtype) for _ in range(2))
+        self.k_scale = self.v_scale = None
+        if fp8:
+            self.k, self.v = ([t.view(engine.kv_dtype) for t in c] for c in (self.k, self.v))
+            self.k_scale, self.v_scale = (make(shape[:-1], torch.uint8) for _ in range(2))
         self.capacity = capacity_blocks
         self.index: OrderedDict[int, int] = OrderedDict()      # content hash -> host slot
         self.free = list(range(capacity_blocks - 1, -1, -1))
@@ -78,7 +101,7 @@ class KVOffloadStore:
             src.append(b)
             dst.append(s)
             keep.append(h)
-        copy_blocks(self.engine.k_cache, self.engine.v_cache, self.k, self.v, src, dst, self.engine.device)
+        copy_cache(self.engine, self, src, dst, self.engine.device)
         for h, s in zip(keep, dst):
             self.index[h] = s
         return len(src)
@@ -92,7 +115,7 @@ class KVOffloadStore:
                 break
             src.append(s)
             dst.append(b)
-        copy_blocks(self.k, self.v, self.engine.k_cache, self.engine.v_cache, src, dst, self.engine.device)
+        copy_cache(self, self.engine, src, dst, self.engine.device)
         return len(src)
 
     def pin(self, hashes) -> None:
@@ -107,7 +130,23 @@ class KVOffloadStore:
         self.free = list(range(self.capacity - 1, -1, -1))
 
 
+def can_transfer(src_engine, dst_engine) -> bool:
+    """Whether :func:`transfer_direct` takes blocks from one engine to the other:
+    caches of one type, or an 8-bit cache to a bf16 one on the same device."""
+    if src_engine.kv_dtype == dst_engine.kv_dtype:
+        return True
+    return src_engine.k_scale is not None and src_engine.device == dst_engine.device
+
+
 def transfer_direct(src_engine, dst_engine, src_blocks: list[int], dst_blocks: list[int]) -> None:
     """Copy KV blocks between two engines (same or peer GPU)."""
-    copy_blocks(src_engine.k_cache, src_engine.v_cache, dst_engine.k_cache, dst_engine.v_cache, src_blocks,
-                dst_blocks, dst_engine.device)
+    if src_engine.kv_dtype == dst_engine.kv_dtype:
+        copy_cache(src_engine, dst_engine, src_blocks, dst_blocks, dst_engine.device)
+        return
+    dev = dst_engine.device
+    src = torch.tensor(src_blocks, dtype=torch.int32, device=dev)
+    dst = torch.tensor(dst_blocks, dtype=torch.int32, device=dev)
+    for cache, scale, out in ((src_engine.k_cache, src_engine.k_scale, dst_engine.k_cache),
+                              (src_engine.v_cache, src_engine.v_scale, dst_engine.v_cache)):
+        for c, e, o in zip(cache, scale, out):
+            ops.read_kv_cache(c, e, src, o, dst)
