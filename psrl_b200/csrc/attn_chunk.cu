@@ -13,15 +13,14 @@
 //    The tiles share every 128-key K/V tile, and the tensor core alternates
 //    between them: S_g = Q_g K^T, softmax of the other tile meanwhile, O_g += P_g V
 //    with P written back to tensor memory over S.
-//      warp 0       Q by TMA
+//      warp 0       TMA: Q, then K/V pages, found through the block table: bf16 ones
+//                   straight into the MMA's tiles (128-byte swizzle); codes, with
+//                   their exponent bytes, into a ring of raw half tiles
 //      warp 1       MMA issuer
 //      warps 4..11  softmax, one thread per row, tiles A and B
-//      warps 12..15 K/V: pages are found through the block table; codes go from
-//                   global memory to registers one tile ahead, become bf16 exactly
-//                   (bits moved into place, times a power of two) and are stored
-//                   in the 128-byte swizzle the MMA reads.  Keys at or past len
-//                   become zeros, whatever their page holds.  bf16 pages are copied
-//                   with cp.async.
+//      warps 12..15 8-bit cache: codes to bf16, exactly (bits moved into place, times
+//                   a power of two), from the raw ring into the MMA's tiles
+//    Values at or past len count as zeros, whatever their page holds.
 //    Registers are moved from the first and last warpgroup to the softmax.
 //  * Few query tiles: the key tiles of a block are split over CTAs, whose partial
 //    rows (fp32, with a base-2 log-sum) a second kernel joins in key order.
@@ -46,7 +45,12 @@ constexpr int BQ = 128, BKV = 128;
 constexpr int ATOM = 128 * 64 * 2;  // 128 rows x 64 bf16 (one 128-byte swizzle atom column)
 constexpr int TILE = 2 * ATOM;      // 32 KB
 constexpr int OFF_K = 2 * TILE, OFF_V = OFF_K + 2 * TILE, OFF_BAR = OFF_V + 2 * TILE;
-constexpr int SMEM = OFF_BAR + 256 + 1024;
+// 8-bit cache: ring of raw half tiles (64 keys): their codes, and per half 64 exponent
+// bytes of K and 64 of V
+constexpr int RK = BKV / 2, RAW = RK * D, NRAW = 4;
+constexpr int OFF_RAW = OFF_BAR + 256, OFF_EXP = OFF_RAW + NRAW * RAW;
+constexpr int smem_bytes(bool fp8) { return (fp8 ? OFF_EXP + NRAW * 2 * RK : OFF_BAR + 256) + 1024; }
+static_assert(smem_bytes(true) <= 227 * 1024, "shared memory of a block");
 constexpr int NTHREADS = 512;
 constexpr float RESCALE_LOG2 = 8.0f;
 
@@ -55,7 +59,6 @@ struct Args {
   const int* kv_lens;
   const int* block_table;
   int64_t bt_row;
-  const uint8_t *k, *v;    // pages: codes or bf16
   const uint8_t *ks, *vs;  // exponent bytes (8-bit cache)
   int64_t num_blocks;
   int T, nq, nkv, group, tok;  // tok: tokens per query tile
@@ -85,13 +88,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// One thread's part of a 128-key tile of codes: rows sub + 16 i, codes 16 c ..
-// of each, and the rows' exponent bytes.
-struct Codes {
-  uint4 w[8];
-  uint32_t e[8];
-};
-
 // Four e4m3 codes as two bf16 pairs holding value * 2^-120 (sign, exponent and
 // mantissa bits moved into place; subnormal codes become subnormal bf16 numbers),
 // times m (a power of two or NaN, in both halves).
@@ -107,7 +103,9 @@ __device__ __forceinline__ void bf16_of4(uint32_t w, uint32_t m, uint32_t* out) 
 }
 
 template <bool FP8>
-__global__ void __launch_bounds__(NTHREADS, 1) chunk_kernel(const __grid_constant__ CUtensorMap tmQ, Args a) {
+__global__ void __launch_bounds__(NTHREADS, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, Args a) {
   const int hk = blockIdx.x, b = blockIdx.y;
   const int blk = a.blocks_z - 1 - (int)blockIdx.z / a.splits, part = (int)blockIdx.z % a.splits;
   const int s0 = max(0, min(a.cu_q[b], a.T)), n = min(a.cu_q[b + 1], a.T) - s0;
@@ -140,8 +138,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk_kernel(const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_BAR);
   const uint32_t bq = smem_u32(bars), bkf = bq + 8, bke = bkf + 16, bvf = bke + 16, bve = bvf + 16, bsf = bve + 16,
-                 bpf = bsf + 16, bof = bpf + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+                 bpf = bsf + 16, bof = bpf + 16, brf = bof + 8, bre = brf + 8 * NRAW;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14 + 2 * NRAW);
   __shared__ volatile int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rows = a.tok * a.group;  // rows of a query tile that hold queries
@@ -149,12 +147,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk_kernel(const __grid_constan
     s_abort = 0;
     mbar_init(bq, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bkf + 8 * i, 4);  // one arrive per K/V warp
-      mbar_init(bvf + 8 * i, 4);
+      mbar_init(bkf + 8 * i, FP8 ? 4 : 1);  // one arrive per converting warp, or the TMA bytes'
+      mbar_init(bvf + 8 * i, FP8 ? 4 : 1);
       mbar_init(bke + 8 * i, 1);
       mbar_init(bve + 8 * i, 1);
       mbar_init(bsf + 8 * i, 1);
       mbar_init(bpf + 8 * i, 4);  // one arrive per softmax warp
+    }
+    for (int i = 0; i < NRAW; ++i) {
+      mbar_init(brf + 8 * i, 33);  // the TMA bytes' arrive and one per lane (exponents)
+      mbar_init(bre + 8 * i, 4);
     }
     mbar_init(bof, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -176,14 +178,70 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk_kernel(const __grid_constan
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    if (warp == 0 && lane == 0 && nK > 0) {
-      tma_prefetch_desc(&tmQ);
-      const uint32_t bytes = (uint32_t)rows * 256;
-      mbar_expect_tx(bq, (nB ? 2 : 1) * bytes);
-      const uint32_t sq = smem_u32(smem);
-      for (int t = 0; t < (nB ? 2 : 1); ++t) {
-        tma_load_3d(sq + t * TILE, &tmQ, 0, hk * a.group, s0 + i0 + t * a.tok, bq);
-        tma_load_3d(sq + t * TILE + ATOM, &tmQ, 64, hk * a.group, s0 + i0 + t * a.tok, bq);
+    if (warp == 0 && nK > 0) {
+      // ----------------------------------------------------------- producer
+      if (lane == 0) {
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+        mbar_expect_tx(bq, (nB ? 2 : 1) * (uint32_t)rows * 256);
+        const uint32_t sq = smem_u32(smem);
+        for (int t = 0; t < (nB ? 2 : 1); ++t) {
+          tma_load_3d(sq + t * TILE, &tmQ, 0, hk * a.group, s0 + i0 + t * a.tok, bq);
+          tma_load_3d(sq + t * TILE + ATOM, &tmQ, 64, hk * a.group, s0 + i0 + t * a.tok, bq);
+        }
+      }
+      const int* bt = a.block_table + (int64_t)b * a.bt_row;
+      const int bs = 1 << a.block_shift;
+      // row of the page tensor that holds the key, or one outside it (TMA fills zeros)
+      auto row_of = [&](int key) {
+        const int p = key < len ? bt[key >> a.block_shift] : -1;
+        return p >= 0 && p < a.num_blocks ? (p * a.nkv + hk) * bs + (key & (bs - 1)) : -BKV;
+      };
+      bool ok = true;
+      if constexpr (FP8) {
+        const int box = min(RK, bs);
+        // step h: half h & 1 of K (h & 2 = 0) or V of entry h / 4
+        for (int h = 0; h < 4 * nK; ++h) {
+          const int st = h % NRAW, key0 = key_tile(h >> 2) * BKV + (h & 1) * RK;
+          if (h >= NRAW) ok = mbar_wait(bre + 8 * st, ((h / NRAW) & 1) ^ 1);
+          if (!__all_sync(0xffffffffu, ok) || s_abort) break;
+          {
+            // exponents: lanes 0..15 four keys of K each, lanes 16..31 of V
+            const int row = row_of(key0 + (lane & 15) * 4);
+            const uint8_t* e = lane < 16 ? a.ks : a.vs;
+            if (row >= 0) e += row;
+            const uint32_t dst = smem_u32(smem) + OFF_EXP + st * 2 * RK + lane * 4;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(e), "r"(row >= 0 ? 4 : 0) : "memory");
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(brf + 8 * st) : "memory");
+          }
+          if (lane == 0) {
+            mbar_expect_tx(brf + 8 * st, RAW);
+            const uint32_t dst = smem_u32(smem) + OFF_RAW + st * RAW;
+            for (int r = 0; r < RK; r += box)
+              tma_load_2d(dst + r * D, (h & 2) ? &tmV : &tmK, 0, row_of(key0 + r), brf + 8 * st);
+          }
+        }
+      } else if (lane == 0) {
+        const int box = min(BKV, bs);
+        for (int u = 0; u < 2 * nK && ok && !s_abort; ++u) {
+          const int j = u >> 1, st = j & 1, key0 = key_tile(j) * BKV;
+          const bool is_v = u & 1;
+          if (j >= 2) ok = mbar_wait((is_v ? bve : bke) + 8 * st, ((j >> 1) & 1) ^ 1);
+          if (!ok) break;
+          const uint32_t fb = (is_v ? bvf : bkf) + 8 * st;
+          mbar_expect_tx(fb, TILE);
+          const uint32_t dst = smem_u32(smem) + (is_v ? OFF_V : OFF_K) + st * TILE;
+          for (int r = 0; r < BKV; r += box) {
+            const int y = row_of(key0 + r);
+            tma_load_2d(dst + r * 128, is_v ? &tmV : &tmK, 0, y, fb);
+            tma_load_2d(dst + ATOM + r * 128, is_v ? &tmV : &tmK, 64, y, fb);
+          }
+        }
+      }
+      if (!ok && lane == 0) {
+        if (!s_abort) set_err(a.err, 55);
+        s_abort = 1;
       }
     } else if (warp == 1 && lane == 0) {
       // --------------------------------------------------------- MMA issuer
@@ -250,126 +308,72 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk_kernel(const __grid_constan
       commit_1cta(bof);
     }
   } else if (warp >= 12) {
-    // -------------------------------------------------------- K / V tiles
+    // ------------------------------------------------- codes to bf16 tiles
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-    const int ct = threadIdx.x - 384;
-    const int* bt = a.block_table + (int64_t)b * a.bt_row;
-    const int bs = 1 << a.block_shift;
-    // page of the 16-key group `lane` (0..7) of list entry j, or -1
-    auto page_of = [&](int j) {
-      const int key = key_tile(j) * BKV + (lane & 7) * 16;
-      if (j >= nK || key >= len) return -1;
-      const int p = bt[key >> a.block_shift];
-      return p >= 0 && p < a.num_blocks ? p : -1;
-    };
-    bool ok = true;
     if constexpr (FP8) {
-      const int sub = ct >> 3, c = ct & 7;
-      // NaN of either vector of a key: through the key's exponent; value codes then read as zeros
-      auto load = [&](bool is_v, int j, int pages, Codes& x) {
-        const int key0 = key_tile(j) * BKV;
+      // a thread converts codes 16c.. of rows sub + 16 i of a half
+      const int ct = threadIdx.x - 384, sub = ct >> 3, c = ct & 7;
+      // the two 16-byte halves in an order that spreads a row's threads over all banks
+      const int first = c >> 2, c0 = 2 * (c & 3);
+      const int to0 = sub * 128 + (((c0 + first) ^ (sub & 7)) << 4), to1 = sub * 128 + (((c0 + 1 - first) ^ (sub & 7)) << 4);
+      // RARE: an exponent that does not fit one bf16 factor (values of 2^16 and more), or keys past len
+      auto convert = [&](auto rare, int h) {
+        constexpr bool RARE = decltype(rare)::value;
+        const bool is_v = h & 2;
+        const int j = h >> 2, st = h % NRAW;
+        const uint8_t* from = smem + OFF_RAW + st * RAW + sub * D + c * 16;
+        const uint8_t* ex = smem + OFF_EXP + st * 2 * RK + sub;
+        uint8_t* tile = smem + (is_v ? OFF_V : OFF_K) + (j & 1) * TILE + (c >> 2) * ATOM + (h & 1) * RK * 128;
+        const int left = len - key_tile(j) * BKV - (h & 1) * RK;  // rows of the half below len
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int pg = __shfl_sync(0xffffffffu, pages, i);
-          const int key = key0 + i * 16 + sub;
-          x.w[i] = make_uint4(0, 0, 0, 0);
-          x.e[i] = 127;
-          if (pg >= 0 && key < len) {
-            const int64_t vec = ((int64_t)pg * a.nkv + hk) * bs + (key & (bs - 1));
-            x.w[i] = *reinterpret_cast<const uint4*>((is_v ? a.v : a.k) + vec * D + c * 16);
-            const uint32_t e = a.ks[vec], f = a.vs[vec];
-            x.e[i] = is_v ? f : (f == 255u ? 255u : e);
-          }
-        }
-      };
-      auto store = [&](bool is_v, int j, const Codes& x) {
-        uint8_t* tile = smem + (is_v ? OFF_V : OFF_K) + (j & 1) * TILE + (c >> 2) * ATOM;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = i * 16 + sub;
-          const uint32_t e = x.e[i];
-          const bool none = e == 255u && is_v;
-          // 2^(e - 127 + 120) where bf16 holds it, else in two factors
-          uint32_t m = e == 255u ? (is_v ? 0u : 0x7fc0u) : min(e + 120u, 254u) << 7;
+        for (int i = 0; i < 4; ++i) {
+          uint4 w = *reinterpret_cast<const uint4*>(from + i * 16 * D);
+          if (RARE && i * 16 + sub >= left) w = make_uint4(0, 0, 0, 0);
+          const uint32_t ek = ex[i * 16], ev = ex[RK + i * 16];
+          const uint32_t e = is_v ? ev : ek;
+          // 2^(e - 127 + 120) where bf16 holds it, else in two factors.  A NaN of either vector
+          // goes through the key; the value's codes then count as zeros
+          uint32_t m = min(e + 120u, 254u) << 7;
+          if (max(ek, ev) == 255u) m = is_v ? (ev == 255u ? 0u : m) : 0x7fc0u;
           m |= m << 16;
           uint32_t out[8];
-          bf16_of4(none ? 0u : x.w[i].x, m, out);
-          bf16_of4(none ? 0u : x.w[i].y, m, out + 2);
-          bf16_of4(none ? 0u : x.w[i].z, m, out + 4);
-          bf16_of4(none ? 0u : x.w[i].w, m, out + 6);
-          if (e > 134u && e < 255u) {
-            uint32_t m2 = (e - 7u) << 7;
+          bf16_of4(w.x, m, out);
+          bf16_of4(w.y, m, out + 2);
+          bf16_of4(w.z, m, out + 4);
+          bf16_of4(w.w, m, out + 6);
+          if constexpr (RARE) {
+            uint32_t m2 = e > 134u && e < 255u ? (e - 7u) << 7 : 0x3f80u;
             m2 |= m2 << 16;
 #pragma unroll
             for (int k = 0; k < 8; ++k) out[k] = mul_bf16x2(out[k], m2);
           }
-          // the two 16-byte halves in an order that spreads a row's threads over all banks
-          const int first = c >> 2, c0 = 2 * (c & 3);
           const uint4 lo = make_uint4(out[0], out[1], out[2], out[3]), hi = make_uint4(out[4], out[5], out[6], out[7]);
-          *reinterpret_cast<uint4*>(tile + r * 128 + (((c0 + first) ^ (r & 7)) << 4)) = first ? hi : lo;
-          *reinterpret_cast<uint4*>(tile + r * 128 + (((c0 + 1 - first) ^ (r & 7)) << 4)) = first ? lo : hi;
+          *reinterpret_cast<uint4*>(tile + to0 + i * 16 * 128) = first ? hi : lo;
+          *reinterpret_cast<uint4*>(tile + to1 + i * 16 * 128) = first ? lo : hi;
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive((is_v ? bvf : bkf) + 8 * (j & 1));
       };
-      Codes kx, vx;
-      int pages = page_of(0);
-      if (nK > 0) load(false, 0, pages, kx);
-      for (int j = 0; j < nK; ++j) {
-        const int next = page_of(j + 1);
-        load(true, j, pages, vx);
-        if (j >= 2) ok = mbar_wait(bke + 8 * (j & 1), ((j >> 1) & 1) ^ 1);
-        if (!__all_sync(0xffffffffu, ok) || s_abort) { ok = false; break; }
-        store(false, j, kx);
-        pages = next;
-        if (j + 1 < nK) load(false, j + 1, pages, kx);
-        if (j >= 2) ok = mbar_wait(bve + 8 * (j & 1), ((j >> 1) & 1) ^ 1);
-        if (!__all_sync(0xffffffffu, ok) || s_abort) { ok = false; break; }
-        store(true, j, vx);
-      }
-    } else {
-      const int sub = ct >> 4, c = ct & 15;
-      // unit u: K of entry u / 2 (even) or V (odd)
-      auto copy = [&](int u, int pages) {
-        const int j = u >> 1, key0 = key_tile(j) * BKV;
-        const uint8_t* src = (u & 1) ? a.v : a.k;
-        const uint32_t tile = smem_u32(smem) + ((u & 1) ? OFF_V : OFF_K) + (j & 1) * TILE + (c >> 3) * ATOM;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = i * 8 + sub, key = key0 + r;
-          const int pg = __shfl_sync(0xffffffffu, pages, i >> 1);
-          const bool in = pg >= 0 && key < len;
-          const uint8_t* p = in ? src + (((int64_t)pg * a.nkv + hk) * bs + (key & (bs - 1))) * (2 * D) + c * 16 : src;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                       "l"(p), "r"(in ? 16 : 0)
-                       : "memory");
+      bool ok = true;
+      for (int h = 0; h < 4 * nK; ++h) {
+        const int j = h >> 2, st = h % NRAW;
+        const bool is_v = h & 2;
+        ok = mbar_wait(brf + 8 * st, (h / NRAW) & 1);
+        if (j >= 2 && !(h & 1)) ok = ok && mbar_wait((is_v ? bve : bke) + 8 * (j & 1), ((j >> 1) & 1) ^ 1);
+        if (!__all_sync(0xffffffffu, ok) || s_abort) {
+          if (lane == 0 && !s_abort) set_err(a.err, 51, h);
+          s_abort = 1;
+          break;
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
-      auto landed = [&](int u) {
-        fence_async_smem();
+        const uint32_t e4 = *reinterpret_cast<const uint32_t*>(smem + OFF_EXP + st * 2 * RK + lane * 4);
+        const bool rare = __vcmpgtu4(e4, 0x86868686u) != 0 || key_tile(j) * BKV + (h & 1) * RK + RK > len;  // 134
+        if (__any_sync(0xffffffffu, rare)) convert(std::true_type{}, h);
+        else convert(std::false_type{}, h);
+        if (h & 1) fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(((u & 1) ? bvf : bkf) + 8 * ((u >> 1) & 1));
-      };
-      int pages = page_of(0);
-      for (int u = 0; u < 2 * nK; ++u) {
-        const int j = u >> 1;
-        if (j >= 2) ok = mbar_wait(((u & 1) ? bve : bke) + 8 * (j & 1), ((j >> 1) & 1) ^ 1);
-        if (!__all_sync(0xffffffffu, ok) || s_abort) { ok = false; break; }
-        copy(u, pages);
-        if (u & 1) pages = page_of(j + 1);
-        if (u > 0) {
-          asm volatile("cp.async.wait_group 1;" ::: "memory");
-          landed(u - 1);
+        if (lane == 0) {
+          mbar_arrive(bre + 8 * st);
+          if (h & 1) mbar_arrive((is_v ? bvf : bkf) + 8 * (j & 1));
         }
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      if (ok && nK > 0) landed(2 * nK - 1);
-    }
-    if (!ok && lane == 0) {
-      if (!s_abort) set_err(a.err, 51);
-      s_abort = 1;
     }
   } else {
     // -------------------------------------------------------------- softmax
@@ -393,6 +397,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk_kernel(const __grid_constan
       }
       fence_after();
       const int key0 = key_tile(j) * BKV;
+      if (!FP8 && key0 + BKV > len) {
+        // bf16 pages came as they are: values past len must be zeros before P V reads them
+        if (!mbar_wait(bvf + 8 * (j & 1), (j >> 1) & 1)) {
+          if (!s_abort) set_err(a.err, 56, j);
+          s_abort = 1;
+          ok = false;
+          break;
+        }
+        uint8_t* tile = smem + OFF_V + (j & 1) * TILE;
+        for (int i = r; i < (key0 + BKV - len) * 16; i += BQ)
+          *reinterpret_cast<uint4*>(tile + (i & 1) * ATOM + (len - key0 + (i >> 4)) * 128 + ((i >> 1) & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+      }
       const int lim = pos - key0;                                   // last key column this row sees
       const int lo = a.window > 0 ? lim - a.window + 1 : 0, sk = a.sinks - key0;  // from lo on, and those before sk
       const bool masked_tile = __any_sync(0xffffffffu, lim < BKV - 1 || (lo > 0 && sk < BKV));
@@ -538,6 +556,22 @@ static CUtensorMap map_q(const at::Tensor& q, int group, int tok) {
   return m;
 }
 
+// bf16 pages as rows of 128: boxes of 64 columns x min(128, block_size) rows.
+static CUtensorMap map_pages(const at::Tensor& t) {
+  CUtensorMap m;
+  const cuuint64_t rows = (cuuint64_t)(t.size(0) * t.size(1) * t.size(2));
+  TORCH_CHECK(rows < (1ull << 31), "cache of more than 2^31 vectors");
+  cuuint64_t dims[2] = {(cuuint64_t)D, rows};
+  cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+  cuuint32_t box[2] = {64u, (cuuint32_t)std::min<int64_t>(BKV, t.size(2))};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = PSRL_DRV(cuTensorMapEncodeTiled)(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, t.data_ptr(), dims, strides,
+                                                box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (", (int)r, ")");
+  return m;
+}
+
 }  // namespace chunk
 
 using namespace chunk;
@@ -576,8 +610,6 @@ at::Tensor attn_paged_chunk(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache
   a.kv_lens = kv_lens.data_ptr<int>();
   a.block_table = block_table.data_ptr<int>();
   a.bt_row = block_table.stride(0);
-  a.k = reinterpret_cast<const uint8_t*>(k_cache.data_ptr());
-  a.v = reinterpret_cast<const uint8_t*>(v_cache.data_ptr());
   a.ks = fp8 ? k_scale->data_ptr<uint8_t>() : nullptr;
   a.vs = fp8 ? v_scale->data_ptr<uint8_t>() : nullptr;
   a.num_blocks = k_cache.size(0);
@@ -595,11 +627,11 @@ at::Tensor attn_paged_chunk(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache
   a.err = err.data_ptr<int>();
   const int64_t per_block = 2 * a.tok;
   a.blocks_z = (int)((std::min(max_q_len, T) + per_block - 1) / per_block);
-  // Split the keys while there are fewer CTAs than SMs: CTAs with work are at most
-  // one per block of tokens; a part keeps four key tiles of the longest context.
+  // Split the keys while the CTAs all fit on the SMs at once: CTAs with work are at
+  // most one per block of tokens; a part keeps four key tiles of the longest context.
   const int64_t ctas = nkv * std::min<int64_t>(B * a.blocks_z, T / per_block + B);
   const int64_t span = window > 0 ? std::min(cap, window + a.sinks + per_block) : cap;
-  int64_t splits = std::min<int64_t>((num_sms() + ctas - 1) / ctas, (span + 4 * BKV - 1) / (4 * BKV));
+  int64_t splits = std::min<int64_t>(num_sms() / ctas, (span + 4 * BKV - 1) / (4 * BKV));
   splits = std::max<int64_t>(1, std::min<int64_t>(splits, 64));
   TORCH_CHECK(a.blocks_z * splits < 65536, "too many query blocks");
   a.splits = (int)splits;
@@ -610,9 +642,12 @@ at::Tensor attn_paged_chunk(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache
     a.part_lse = a.part_o + splits * T * nq * D;
   }
   const CUtensorMap tq = map_q(q, a.group, a.tok);
+  const CUtensorMap tk = fp8 ? kv8::map_codes(k_cache, RK, CU_TENSOR_MAP_SWIZZLE_NONE) : map_pages(k_cache);
+  const CUtensorMap tv = fp8 ? kv8::map_codes(v_cache, RK, CU_TENSOR_MAP_SWIZZLE_NONE) : map_pages(v_cache);
   auto* kern = fp8 ? chunk_kernel<true> : chunk_kernel<false>;
-  ensure_smem_attr(kern, SMEM);
-  kern<<<dim3((unsigned)nkv, (unsigned)B, (unsigned)(a.blocks_z * splits)), NTHREADS, SMEM, stream()>>>(tq, a);
+  ensure_smem_attr(kern, smem_bytes(fp8));
+  kern<<<dim3((unsigned)nkv, (unsigned)B, (unsigned)(a.blocks_z * splits)), NTHREADS, smem_bytes(fp8), stream()>>>(tq, tk, tv,
+                                                                                                                        a);
   PSRL_CHECK_LAUNCH();
   if (splits > 1) {
     chunk_join<<<(unsigned)((T * nq * 32 + 255) / 256), 256, 0, stream()>>>(a, (int)B);

@@ -15,18 +15,20 @@
 //  * A producer warp keeps NS tiles (K, V: TMA boxes with the 128-byte swizzle;
 //    exponent bytes: 4-byte cp.async) in flight over an mbarrier ring, across
 //    pair boundaries.
-//  * Four consumer warps take 16 keys of each tile.  The m16n8k16 fragments come
-//    straight out of the swizzled tile with conflict-free 16-byte loads: the
-//    contraction order over d and the output order over d are permuted so that
-//    a thread's fragment is the 32 consecutive codes 32t.. of key g (K) and the
-//    16 consecutive codes 16g.. of keys 2t, 2t+1, 2t+8, 2t+9 (V).
-//  * e4m3 -> f16 is a shift and two masks per pair: the code's sign, exponent and
-//    mantissa bits moved into place are the value times 2^-8, subnormals
-//    included; 2^8 joins the scale.  f16 products with fp32 accumulation: the
-//    codes are exact in f16, a query row is scaled by a power of two so that its
-//    largest value is in [2^14, 2^15) (its bf16 values are then exact in f16 down
-//    to 2^-31 of the largest), and the probabilities keep f16's 11 bits.
-//  * The exponents cost nothing per element: 2^ek scales a column of S, and
+//  * Four consumer warps take 16 keys of each tile.  The products are taken
+//    transposed, S^T = K Q^T and O^T += V^T P^T, so that the 16 rows of an
+//    m16n8k16 are keys (columns of V) and its 8 columns the query heads of the
+//    group: groups of up to 8 heads waste nothing (NT = 1), 9 to 16 take two
+//    column tiles.  P^T gets from accumulator to operand layout with movmatrix.
+//  * Fragments come straight out of the swizzled tile with conflict-free 16-byte
+//    loads: the contraction order over d and the output order over d are permuted
+//    so that a thread's fragment is the 32 consecutive codes 32t.. of keys g and
+//    g+8 (K) and the 16 consecutive codes 16g.. of keys 2t, 2t+1, 2t+8, 2t+9 (V).
+//  * e4m3 -> f16 is one conversion per pair, exact; f16 products with fp32
+//    accumulation.  A query row is scaled by a power of two so that its largest
+//    value is in [2^14, 2^15) (its bf16 values are then exact in f16 down to 2^-31
+//    of the largest), and the probabilities keep f16's 11 bits.
+//  * The exponents cost nothing per element: 2^ek scales a row of S^T, and
 //    P 2^ev is the second product's operand, with the running maximum taken over
 //    log2(p) + ev so that it stays within f16's range.
 #include "checks.cuh"
@@ -42,12 +44,12 @@ using namespace tc5;
 
 constexpr int D = 128;
 constexpr int TK = 64;                        // keys per tile
-constexpr int NS = 4;                         // ring depth
+constexpr int NS = 3;                         // ring depth
 constexpr int TILE = TK * D;                  // 8 KB of codes
 constexpr int STAGE = 2 * TILE;               // K, V
 constexpr int OFF_EXP = NS * STAGE;           // per stage: 64 K exponents, 64 V exponents
 constexpr int OFF_MERGE = OFF_EXP + NS * 2 * TK;
-constexpr int MROW = 136;                     // merge row pitch in floats (conflict-free float2 stores)
+constexpr int MROW = 132;                     // merge row pitch in floats (conflict-free float2 stores)
 constexpr int NTHREADS = 160;                 // 4 consumer warps + producer
 constexpr float GROW = 8.0f;                  // rescale O when the running maximum grows by more than 2^8
 
@@ -85,10 +87,17 @@ __device__ __forceinline__ Tiles tiles_of(const Args& a, int b) {
 }
 
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// an 8 x 8 matrix of 16-bit values, a row per four lanes, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
 }
 
 // Block-wide scan over the sequences: returns the number of items (tiles of all
@@ -123,7 +132,11 @@ __device__ __forceinline__ int64_t share_of(int64_t total, int workers) {
   return max((int64_t)1, (total + workers - 1) / workers);
 }
 
-__global__ void __launch_bounds__(NTHREADS, 2)
+constexpr int smem_bytes(int nt) { return OFF_MERGE + 4 * 8 * nt * MROW * 4 + 1024; }
+constexpr int resident(int nt) { return nt == 1 ? 3 : 2; }  // CTAs per SM
+
+template <int NT>
+__global__ void __launch_bounds__(NTHREADS, resident(NT))
     decode8_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -233,48 +246,62 @@ __global__ void __launch_bounds__(NTHREADS, 2)
   const int g = lane >> 2, t = lane & 3;
   const int grp = a.nq / a.nkv;
   float* merge = reinterpret_cast<float*>(smem + OFF_MERGE);
+  const int base = warp * 16;  // this warp's keys of a tile
+  // offsets within a tile of this thread's K rows g, g+8 (16-byte chunks 2t, 2t+1) and
+  // V rows 2t, 2t+1, 2t+8, 2t+9 (chunk g); row & 7 does not depend on the warp
+  const int ko = (base + g) * D + (((2 * t) ^ g) << 4);
+  const int v0o = (base + 2 * t) * D + ((g ^ (2 * t)) << 4), v1o = (base + 2 * t + 1) * D + ((g ^ (2 * t + 1)) << 4);
   int it = 0;
   bool ok = true;
   while (it < count) {
     const int seg0 = i, seg = min(tl.n - i, count - it);  // tiles of this pair in this share
-    // queries: fragment words of step s hold d = 32t + 4s + {0, 2} and {1, 3}
-    uint32_t qf[8][4];
-    float fr[2];  // row factor: scale * log2(e), f16 scaling of the row and 2^8 of the codes
+    // queries: head 8u + g, the fragment words of step k hold d = 32t + 4k + {0, 1} and {2, 3}
+    uint32_t qf[NT][8][2];
+    float fr[NT][2];  // heads 8u + 2t, +1: scale * log2(e) and the f16 scaling of the head's query
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = g + 8 * r;
+    for (int u = 0; u < NT; ++u) {
+      const int head = 8 * u + g;
       uint4 w[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         w[c] = make_uint4(0, 0, 0, 0);
-        if (row < grp)
-          w[c] = *reinterpret_cast<const uint4*>(a.q + (int64_t)b * a.q_row + (int64_t)(hk * grp + row) * D + 32 * t +
+        if (head < grp)
+          w[c] = *reinterpret_cast<const uint4*>(a.q + (int64_t)b * a.q_row + (int64_t)(hk * grp + head) * D + 32 * t +
                                                  8 * c);
       }
-      const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
+      const uint32_t* x = reinterpret_cast<const uint32_t*>(w);
       uint32_t m = 0;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) m = __vmaxu2(m, u[k] & 0x7fff7fffu);
+      for (int k = 0; k < 16; ++k) m = __vmaxu2(m, x[k] & 0x7fff7fffu);
       m = max(m & 0xffffu, m >> 16);
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      // 2^(14 - E) for a largest value in [2^E, 2^(E+1)), in two factors that stay finite
+      // 2^(14 - E) for a largest value in [2^E, 2^(E+1)); both it and its inverse stay finite
       const int up = min(max(14 - ((int)(m >> 7) - 127), -113), 126);
       const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-      fr[r] = a.scale_log2 * 256.f * __uint_as_float((uint32_t)(127 - up) << 23);
+      const float back = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+      fr[u][0] = __shfl_sync(0xffffffffu, back, 8 * t);      // from the lanes of head 2t
+      fr[u][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);  // and 2t + 1
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const float2 x = __bfloat1622float2(*reinterpret_cast<const bf162*>(u + 2 * s));
-        const float2 y = __bfloat1622float2(*reinterpret_cast<const bf162*>(u + 2 * s + 1));
-        const half2 e = __floats2half2_rn(x.x * f, y.x * f), od = __floats2half2_rn(x.y * f, y.y * f);
-        qf[s][r] = *reinterpret_cast<const uint32_t*>(&e);
-        qf[s][2 + r] = *reinterpret_cast<const uint32_t*>(&od);
-      }
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float2 y = __bfloat1622float2(*reinterpret_cast<const bf162*>(x + 2 * k + c));
+          const half2 h = __floats2half2_rn(y.x * f, y.y * f);
+          qf[u][k][c] = *reinterpret_cast<const uint32_t*>(&h);
+        }
     }
-    float o[16][4];
+    float o[NT][8][4];  // rows d = 16g + 2k, + 1; columns heads 8u + 2t, + 1
 #pragma unroll
-    for (int k = 0; k < 16; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
-    float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.f, 0.f};
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[u][k][0] = o[u][k][1] = o[u][k][2] = o[u][k][3] = 0.f;
+    float m_r[NT][2], l_r[NT][2];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      m_r[u][0] = m_r[u][1] = -INFINITY;
+      l_r[u][0] = l_r[u][1] = 0.f;
+    }
 
     for (int e = 0; e < seg; ++e, ++it, ++i) {
       const int st = it % NS;
@@ -285,142 +312,159 @@ __global__ void __launch_bounds__(NTHREADS, 2)
       }
       const uint8_t* kt = smem + st * STAGE;
       const uint8_t* vt = kt + TILE;
-      const uint8_t* ex = smem + OFF_EXP + st * 2 * TK;
-      const int base = warp * 16;
-      float s[2][4];
+      const uint8_t* ex = smem + OFF_EXP + st * 2 * TK + base;
+      uint32_t ka[8], kb[8];  // codes of keys g and g + 8
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
-        const int row = base + u * 8 + g;
-        uint32_t w[8];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          *reinterpret_cast<uint4*>(w + 4 * c) =
-              *reinterpret_cast<const uint4*>(kt + row * D + (((2 * t + c) ^ (row & 7)) << 4));
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mma_f16(s[u], qf[k], kv8::f16_even(w[k]), kv8::f16_odd(w[k]));
+      for (int c = 0; c < 2; ++c) {
+        *reinterpret_cast<uint4*>(ka + 4 * c) = *reinterpret_cast<const uint4*>(kt + (ko ^ (c << 4)));
+        *reinterpret_cast<uint4*>(kb + 4 * c) = *reinterpret_cast<const uint4*>(kt + 8 * D + (ko ^ (c << 4)));
       }
-      // V codes early: their loads overlap the softmax
-      uint4 vw[4];
+      const uint32_t ek0 = ex[g], ek1 = ex[g + 8], ev0 = ex[TK + g], ev1 = ex[TK + g + 8];
+      uint32_t v[4][4];
+      *reinterpret_cast<uint4*>(v[0]) = *reinterpret_cast<const uint4*>(vt + v0o);
+      *reinterpret_cast<uint4*>(v[1]) = *reinterpret_cast<const uint4*>(vt + v1o);
+      *reinterpret_cast<uint4*>(v[2]) = *reinterpret_cast<const uint4*>(vt + 8 * D + v0o);
+      *reinterpret_cast<uint4*>(v[3]) = *reinterpret_cast<const uint4*>(vt + 8 * D + v1o);
+      float s[NT][4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int row = base + 2 * t + (c & 1) + (c >> 1) * 8;
-        vw[c] = *reinterpret_cast<const uint4*>(vt + row * D + ((g ^ (row & 7)) << 4));
+      for (int u = 0; u < NT; ++u) s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t f[4] = {kv8::f16_of2(ka[k]), kv8::f16_of2(kb[k]), kv8::f16_of2_hi(ka[k]), kv8::f16_of2_hi(kb[k])};
+#pragma unroll
+        for (int u = 0; u < NT; ++u) mma_f16(s[u], f, qf[u][k][0], qf[u][k][1]);
       }
-      const int key0 = tl.key0(i) + base + 2 * t;
-      float y[2][4], x[2][4], inv[2][2];
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t ek2 = *reinterpret_cast<const uint16_t*>(ex + base + u * 8 + 2 * t);
-        const uint32_t ev2 = *reinterpret_cast<const uint16_t*>(ex + TK + base + u * 8 + 2 * t);
+      float kf[2] = {__uint_as_float(ek0 << 23), __uint_as_float(ek1 << 23)};         // 2^ek
+      float vf[2] = {(float)((int)ev0 - 127), (float)((int)ev1 - 127)};               // ev
+      // keys outside the context or the window, and exponents of 255: rare tiles
+      const int tile0 = tl.key0(i) + base;
+      const bool edge = tile0 + 16 > tl.len || (tile0 < tl.lo && tile0 + 16 > a.sinks);
+      if (__any_sync(0xffffffffu, edge || max(max(ek0, ek1), max(ev0, ev1)) == 255u)) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int key = key0 + u * 8 + c;
-          const bool see = key < tl.len && (key >= tl.lo || key < a.sinks);
-          const uint32_t ek = (ek2 >> (8 * c)) & 255u, ev = (ev2 >> (8 * c)) & 255u;
-          const float kf = kv8::exp2_byte(ek);
-          const float vf = ev == 255u ? NAN : (float)((int)ev - 127);
-          inv[u][c] = __uint_as_float((254u - min(ev, 253u)) << 23);  // 2^-(ev - 127)
+          const int key = tile0 + g + 8 * c;
+          if (!(key < tl.len && (key >= tl.lo || key < a.sinks))) {
+            kf[c] = 1.f;
+            vf[c] = 0.f;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            x[u][2 * r + c] = see ? s[u][2 * r + c] * (fr[r] * kf) : -INFINITY;
-            y[u][2 * r + c] = see ? x[u][2 * r + c] + vf : -INFINITY;
-            top[r] = fmaxf(top[r], y[u][2 * r + c]);
+            for (int u = 0; u < NT; ++u) s[u][2 * c] = s[u][2 * c + 1] = -INFINITY;
+          } else if ((c ? ek1 : ek0) == 255u || (c ? ev1 : ev0) == 255u) {
+            kf[c] = vf[c] = NAN;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          // whatever the page holds in rows nobody sees: 0 * NaN would be one
+          const int key = tile0 + 2 * t + (c & 1) + 8 * (c >> 1);
+          if (!(key < tl.len && (key >= tl.lo || key < a.sinks))) v[c][0] = v[c][1] = v[c][2] = v[c][3] = 0;
+        }
+      }
+      float y[NT][4], f[NT][4], top[NT][2];
+      bool grow = false;
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f[u][k] = fr[u][k & 1] * kf[k >> 1];
+          y[u][k] = fmaf(s[u][k], f[u][k], vf[k >> 1]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float m = fmaxf(y[u][c], y[u][2 + c]);
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          top[u][c] = m;
+          grow |= m > m_r[u][c] + GROW || (m_r[u][c] == -INFINITY && m > m_r[u][c]);
+        }
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          float corr[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float mn = fmaxf(m_r[u][c], top[u][c]);
+            corr[c] = m_r[u][c] == -INFINITY ? 0.f : ex2(m_r[u][c] - mn);
+            m_r[u][c] = mn;
+            l_r[u][c] *= corr[c];
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            o[u][k][0] *= corr[0];
+            o[u][k][1] *= corr[1];
+            o[u][k][2] *= corr[0];
+            o[u][k][3] *= corr[1];
           }
         }
       }
+      uint32_t pf[NT][2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      }
-      const bool grow = top[0] > m_r[0] + GROW || top[1] > m_r[1] + GROW || (m_r[0] == -INFINITY && top[0] > m_r[0]) ||
-                        (m_r[1] == -INFINITY && top[1] > m_r[1]);
-      if (__any_sync(0xffffffffu, grow)) {
-        float corr[2];
+      for (int u = 0; u < NT; ++u) {
+        const float r0 = m_r[u][0] == -INFINITY ? 0.f : m_r[u][0], r1 = m_r[u][1] == -INFINITY ? 0.f : m_r[u][1];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float mn = fmaxf(m_r[r], top[r]);
-          corr[r] = m_r[r] == -INFINITY ? 0.f : ex2(m_r[r] - mn);
-          m_r[r] = mn;
-          l_r[r] *= corr[r];
-        }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          o[k][0] *= corr[0];
-          o[k][1] *= corr[0];
-          o[k][2] *= corr[1];
-          o[k][3] *= corr[1];
+        for (int c = 0; c < 2; ++c) {  // keys g, g + 8
+          const half2 h = __floats2half2_rn(ex2(y[u][2 * c] - r0), ex2(y[u][2 * c + 1] - r1));
+          l_r[u][0] += ex2(fmaf(s[u][2 * c], f[u][2 * c], -r0));
+          l_r[u][1] += ex2(fmaf(s[u][2 * c + 1], f[u][2 * c + 1], -r1));
+          pf[u][c] = transpose8(*reinterpret_cast<const uint32_t*>(&h));
         }
       }
-      uint32_t pf[4];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float ref = m_r[r] == -INFINITY ? 0.f : m_r[r];
-          const float w0 = ex2(y[u][2 * r] - ref), w1 = ex2(y[u][2 * r + 1] - ref);
-          l_r[r] = fmaf(w0, inv[u][0], l_r[r]);
-          l_r[r] = fmaf(w1, inv[u][1], l_r[r]);
-          const half2 h = __floats2half2_rn(w0, w1);
-          pf[2 * u + r] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vw[0]);
-      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vw[1]);
-      const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vw[2]);
-      const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vw[3]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t a01 = __byte_perm(v0[k], v1[k], 0x5410), a23 = __byte_perm(v0[k], v1[k], 0x7632);
-        const uint32_t b01 = __byte_perm(v2[k], v3[k], 0x5410), b23 = __byte_perm(v2[k], v3[k], 0x7632);
-        mma_f16(o[4 * k], pf, kv8::f16_even(a01), kv8::f16_even(b01));
-        mma_f16(o[4 * k + 1], pf, kv8::f16_odd(a01), kv8::f16_odd(b01));
-        mma_f16(o[4 * k + 2], pf, kv8::f16_even(a23), kv8::f16_even(b23));
-        mma_f16(o[4 * k + 3], pf, kv8::f16_odd(a23), kv8::f16_odd(b23));
+        // codes of two keys side by side, for one column of V after the other
+        const uint32_t a01 = __byte_perm(v[0][k], v[1][k], 0x5140), a23 = __byte_perm(v[0][k], v[1][k], 0x7362);
+        const uint32_t b01 = __byte_perm(v[2][k], v[3][k], 0x5140), b23 = __byte_perm(v[2][k], v[3][k], 0x7362);
+        const uint32_t f0[4] = {kv8::f16_of2(a01), kv8::f16_of2_hi(a01), kv8::f16_of2(b01), kv8::f16_of2_hi(b01)};
+        const uint32_t f1[4] = {kv8::f16_of2(a23), kv8::f16_of2_hi(a23), kv8::f16_of2(b23), kv8::f16_of2_hi(b23)};
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          mma_f16(o[u][2 * k], f0, pf[u][0], pf[u][1]);
+          mma_f16(o[u][2 * k + 1], f1, pf[u][0], pf[u][1]);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + 8 * st);
     }
-    if (!ok) {
-      if (lane == 0) {
-        if (!s_abort && a.err) atomicCAS(a.err, 0, 42);
-        s_abort = 1;
-        s_fail = 1;
-      }
+    if (!ok && lane == 0) {
+      if (!s_abort && a.err) atomicCAS(a.err, 0, 42);
+      s_abort = 1;
+      s_fail = 1;
     }
     // ------------------------------------------------- join the four warps
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l_r[r] += __shfl_xor_sync(0xffffffffu, l_r[r], 1);
-      l_r[r] += __shfl_xor_sync(0xffffffffu, l_r[r], 2);
-      if (t == 0) {
-        s_m[warp][g + 8 * r] = m_r[r];
-        s_l[warp][g + 8 * r] = l_r[r];
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l_r[u][c] += __shfl_xor_sync(0xffffffffu, l_r[u][c], x);
+        if (g == 0) {
+          s_m[warp][8 * u + 2 * t + c] = m_r[u][c];
+          s_l[warp][8 * u + 2 * t + c] = l_r[u][c];
+        }
       }
-    }
     asm volatile("bar.sync 1, 128;" ::: "memory");
     if (s_fail) return;  // uniform: not written between this barrier and the next
-    float mg[2], cw[2];
+    // columns d = 16g + 2k, + 1 of a head's output sit at 16k + 2g
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = g + 8 * r;
-      mg[r] = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
-      cw[r] = m_r[r] == -INFINITY ? 0.f : ex2(m_r[r] - mg[r]);
-    }
-    // column d = 16n + k of the tile's output sits at 8k + n
+    for (int u = 0; u < NT; ++u)
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
+      for (int c = 0; c < 2; ++c) {
+        const int row = 8 * u + 2 * t + c;
+        const float mg = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+        const float cw = m_r[u][c] == -INFINITY ? 0.f : ex2(m_r[u][c] - mg);
+        if (row < grp) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-        if (g + 8 * r < grp)
-          *reinterpret_cast<float2*>(merge + (warp * 16 + g + 8 * r) * MROW + 8 * k + 2 * t) =
-              make_float2(o[k][2 * r] * cw[r], o[k][2 * r + 1] * cw[r]);
+          for (int k = 0; k < 8; ++k)
+            *reinterpret_cast<float2*>(merge + (warp * 8 * NT + row) * MROW + 16 * k + 2 * g) =
+                make_float2(o[u][k][c] * cw, o[u][k][2 + c] * cw);
+        }
+      }
     asm volatile("bar.sync 1, 128;" ::: "memory");
     const bool whole = seg0 == 0 && seg == tl.n;
     const int64_t slot = 2 * (int64_t)blockIdx.x + (it == seg ? 0 : 1);  // the share's first pair, or its last
     for (int idx = threadIdx.x; idx < grp * D; idx += 128) {
-      const int row = idx / D, d = idx % D, p = 8 * (d & 15) + (d >> 4);
+      const int row = idx / D, d = idx % D, p = 16 * ((d >> 1) & 7) + 2 * (d >> 4) + (d & 1);
       float m = s_m[0][row];
 #pragma unroll
       for (int w = 1; w < 4; ++w) m = fmaxf(m, s_m[w][row]);
@@ -428,10 +472,10 @@ __global__ void __launch_bounds__(NTHREADS, 2)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         l += s_m[w][row] == -INFINITY ? s_l[w][row] : s_l[w][row] * ex2(s_m[w][row] - m);
-        acc += merge[(w * 16 + row) * MROW + p];
+        acc += merge[(w * 8 * NT + row) * MROW + p];
       }
       // a NaN anywhere in the row's sums stays a NaN; nothing visible gives zeros
-      const float val = l == 0.f ? 0.f : acc * 256.f / l;
+      const float val = l == 0.f ? 0.f : acc / l;
       if (whole) {
         a.o[((int64_t)b * a.nq + hk * grp + row) * D + d] = __float2bfloat16(val);
       } else {
@@ -542,7 +586,8 @@ at::Tensor attn_decode_fp8(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
   const int64_t cap = block_table.size(1) * k_cache.size(2);
   TORCH_CHECK(cap < (1ll << 31) && B * nq < (1ll << 31), "block table too wide");
   if (cap == 0 || k_cache.size(0) == 0) return o.zero_();
-  const CUtensorMap tk = kv8::map_codes(k_cache, TK), tv = kv8::map_codes(v_cache, TK);
+  const CUtensorMap tk = kv8::map_codes(k_cache, TK, CU_TENSOR_MAP_SWIZZLE_128B),
+                    tv = kv8::map_codes(v_cache, TK, CU_TENSOR_MAP_SWIZZLE_128B);
   Args a{};
   a.q = reinterpret_cast<const bf16*>(q.data_ptr());
   a.q_row = q.stride(0);
@@ -562,16 +607,18 @@ at::Tensor attn_decode_fp8(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.o = reinterpret_cast<bf16*>(o.data_ptr());
   a.err = err.data_ptr<int>();
-  // two CTAs fit an SM; never more of them than tiles there can be
+  // one column tile of up to 8 heads leaves room for three CTAs on an SM; never
+  // more of them than tiles there can be
+  const int nt = nq / nkv <= 8 ? 1 : 2;
   const int64_t most = B * nkv * ((cap + TK - 1) / TK);
-  a.workers = (int)std::min<int64_t>(2 * num_sms(), most);
+  a.workers = (int)std::min<int64_t>(resident(nt) * num_sms(), most);
   auto part = at::empty({2 * a.workers * 16 * (D + 1)}, q.options().dtype(at::kFloat));
   a.part_o = part.data_ptr<float>();
   a.part_lse = a.part_o + 2ll * a.workers * 16 * D;
-  constexpr int SMEM = OFF_MERGE + 64 * MROW * 4 + 1024;
-  static_assert(2 * (SMEM + 2048) <= 228 * 1024, "two CTAs per SM");
-  ensure_smem_attr(decode8_kernel, SMEM);
-  decode8_kernel<<<a.workers, NTHREADS, SMEM, stream()>>>(tk, tv, a);
+  static_assert(3 * (smem_bytes(1) + 2048) <= 228 * 1024 && 2 * (smem_bytes(2) + 2048) <= 228 * 1024, "resident CTAs");
+  auto* kern = nt == 1 ? decode8_kernel<1> : decode8_kernel<2>;
+  ensure_smem_attr(kern, smem_bytes(nt));
+  kern<<<a.workers, NTHREADS, smem_bytes(nt), stream()>>>(tk, tv, a);
   PSRL_CHECK_LAUNCH();
   decode8_join<<<(unsigned)(B * nq), 128, 0, stream()>>>(a);
   PSRL_CHECK_LAUNCH();

@@ -11,20 +11,22 @@
 namespace psrl {
 namespace kv8 {
 
-// e4m3 codes in bytes 0 and 2 (even) or 1 and 3 (odd) of w as two f16 holding
-// the codes' values times 2^-8: sign to bit 15, exponent and mantissa to bits
-// 13..7.  Subnormal codes become subnormal f16 numbers, exactly.
-__device__ __forceinline__ uint32_t f16_odd(uint32_t w) { return (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u); }
-__device__ __forceinline__ uint32_t f16_even(uint32_t w) { return f16_odd(w << 8); }
-
-// 2^(byte - 127); byte 255 is a NaN, byte 0 (never written) counts as zero
-__device__ __forceinline__ float exp2_byte(uint32_t byte) {
-  return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
+// Two e4m3 codes (low byte first) as two f16, exactly; codes 0x7f and 0xff are NaN.
+__device__ __forceinline__ uint32_t f16_of2(uint32_t codes) {
+  uint32_t r;
+  asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;\n}" : "=r"(r) : "r"(codes));
+  return r;
+}
+// The same for the high half of a word.
+__device__ __forceinline__ uint32_t f16_of2_hi(uint32_t codes) {
+  uint32_t r;
+  asm("{\n .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, hi;\n}" : "=r"(r) : "r"(codes));
+  return r;
 }
 
 // Tensor map over the codes: rows of 128 bytes (one vector each), boxes of
-// min(tile, block_size) rows, 128-byte swizzle.
-inline CUtensorMap map_codes(const at::Tensor& t, int tile) {
+// min(tile, block_size) rows.
+inline CUtensorMap map_codes(const at::Tensor& t, int tile, CUtensorMapSwizzle swizzle) {
   CUtensorMap m;
   const cuuint64_t rows = (cuuint64_t)(t.size(0) * t.size(1) * t.size(2));
   TORCH_CHECK(rows < (1ull << 31), "cache of more than 2^31 vectors");
@@ -33,7 +35,7 @@ inline CUtensorMap map_codes(const at::Tensor& t, int tile) {
   cuuint32_t box[2] = {128u, (cuuint32_t)std::min<int64_t>(tile, t.size(2))};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = PSRL_DRV(cuTensorMapEncodeTiled)(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, t.data_ptr(), dims, strides, box,
-                                                estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (", (int)r, ")");
   return m;
