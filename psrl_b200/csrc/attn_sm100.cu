@@ -75,6 +75,7 @@ struct FwdArgs {
   int64_t o_row;
   float* lse;        // [nq, T] natural log, or null
   int window, sinks; // WIN only
+  bf16* o_lo;        // WIN, or null: what o's rounding left out, [T, nq * D]
   int* err;
 };
 
@@ -273,7 +274,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const int r = quad * 32 + lane;           // row within the tile
     const int row_pos = q0 + g * BQ + r;      // position within the sequence
     const uint32_t ts = tS(g) + ((uint32_t)(quad * 32) << 16), to = tO(g) + ((uint32_t)(quad * 32) << 16);
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, lb = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       if (!mbar_wait(bsf + 8 * g, j & 1) || s_abort) {
@@ -323,8 +324,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         m = m_new;
       }
       const float ref = (m == -INFINITY) ? 0.f : m;
-      // pass 2: P = 2^(x - ref) in bf16, packed two per column over S's first 64 columns
-      float ls0 = 0.f, ls1 = 0.f;
+      // pass 2: P = 2^(x - ref) in bf16, packed two per column over S's first 64 columns.
+      // WIN: lr sums the rounded P, which O is divided by, so that the weights of a
+      // row add up to one; the log-sum-exp keeps the unrounded sum l
+      float ls0 = 0.f, ls1 = 0.f, lr0 = 0.f, lr1 = 0.f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t pk[16];
@@ -338,6 +341,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           ls1 += p1;
           const bf162 pp = __floats2bfloat162_rn(p0, p1);
           pk[i] = *reinterpret_cast<const uint32_t*>(&pp);
+          if (WIN) {
+            lr0 += __uint_as_float(pk[i] << 16);
+            lr1 += __uint_as_float(pk[i] & 0xffff0000u);
+          }
         }
         tmem_st16(ts + c * 16, pk);
       }
@@ -356,6 +363,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
       }
       l = l * alpha + (ls0 + ls1);
+      if (WIN) lb = lb * alpha + (lr0 + lr1);
       tmem_wait_st();
       fence_before();
       __syncwarp();
@@ -366,7 +374,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       fence_after();
       if (ok && !s_abort) {
         const bool valid = row_pos < L;
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float den = WIN ? lb : l;
+        const float inv = den > 0.f ? 1.f / den : 0.f;
         bf16* orow = a.o + (int64_t)(s0 + row_pos) * a.o_row + (int64_t)h * D;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
@@ -379,6 +388,13 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]) * inv;
 #pragma unroll
             for (int i = 0; i < 32; i += 8) *reinterpret_cast<bf16x8*>(orow + c * 32 + i) = pack8(f + i);
+            if (WIN && a.o_lo != nullptr) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) f[i] -= __bfloat162float(__float2bfloat16(f[i]));
+              bf16* lrow = a.o_lo + (orow - a.o) + c * 32;
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) *reinterpret_cast<bf16x8*>(lrow + i) = pack8(f + i);
+            }
           }
         }
         if (valid && a.lse != nullptr)
@@ -443,7 +459,9 @@ struct BwdArgs {
   int* err;
 };
 
-__global__ void fa_bwd_dot(const bf16* __restrict__ o, const bf16* __restrict__ dout, int64_t T, int nq,
+// o_lo (or null): what o's rounding to bf16 left out; D is then as exact as P, dP
+// are (an error of D is common to a row's dS and does not average out over its keys)
+__global__ void fa_bwd_dot(const bf16* __restrict__ o, const bf16* __restrict__ o_lo, const bf16* __restrict__ dout, int64_t T, int nq,
                            float* __restrict__ dd, const int* __restrict__ cu_end, bf16* __restrict__ dq,
                            int64_t dq_row, int dq_col, bf16* __restrict__ dkv, int64_t dkv_row, int dkv_cols) {
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
@@ -465,6 +483,11 @@ __global__ void fa_bwd_dot(const bf16* __restrict__ o, const bf16* __restrict__ 
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) s += __bfloat162float(po[i]) * __bfloat162float(pd[i]);
+  if (o_lo) {
+    const bf16* pl = o_lo + w * D + lane * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += __bfloat162float(pl[i]) * __bfloat162float(pd[i]);
+  }
   s = warp_sum(s);
   if (lane == 0) dd[(int64_t)h * T + t] = s;
 }
@@ -1087,7 +1110,8 @@ static std::vector<at::Tensor> fwd_launch(const at::Tensor& q, const at::Tensor&
   at::cuda::CUDAGuard g(q.device());
   auto o = at::empty({T, nq * D}, q.options());
   auto lse = want_lse ? at::empty({nq, T}, q.options().dtype(at::kFloat)) : at::Tensor();
-  if (T == 0 || B <= 0 || max_q <= 0) return {window > 0 ? o.zero_() : o, lse};
+  auto o_lo = want_lse && window > 0 ? at::empty({T, nq * D}, q.options()) : at::Tensor();
+  if (T == 0 || B <= 0 || max_q <= 0) return {window > 0 ? o.zero_() : o, lse, o_lo};
   const CUtensorMap tq = map_rows_64x128(q), tkv = map_rows_64x128(kv);
   FwdArgs a{};
   a.cu = cu_q.data_ptr<int>();
@@ -1106,17 +1130,20 @@ static std::vector<at::Tensor> fwd_launch(const at::Tensor& q, const at::Tensor&
   a.err = err.data_ptr<int>();
   a.window = (int)window;
   a.sinks = (int)sinks;
+  a.o_lo = o_lo.defined() ? reinterpret_cast<bf16*>(o_lo.data_ptr()) : nullptr;
   auto* kern = window > 0 ? fa_fwd_kernel<true> : fa_fwd_kernel<false>;
   ensure_smem_attr(kern, SMEM_BYTES);
   dim3 grid((unsigned)nq, (unsigned)B, (unsigned)a.blocks_z);
   kern<<<grid, NTHREADS, SMEM_BYTES, stream()>>>(tq, tkv, a);
   PSRL_CHECK_LAUNCH();
-  return {o, lse};
+  return {o, lse, o_lo};
 }
 
 // qkv: [T, (nq + 2 nkv) * 128] bf16 (q heads, then k heads, then v heads per
 // token, unit inner stride, rows on 16-byte boundaries).  Returns
-// {o [T, nq * 128] bf16, lse [nq, T] fp32 (natural log; empty unless want_lse)}.
+// {o [T, nq * 128] bf16, lse [nq, T] fp32 (natural log; empty unless want_lse), and
+// with both want_lse and a window o's rounding residue [T, nq * 128] bf16 for the
+// backward}.
 std::vector<at::Tensor> attn_fwd_sm100(at::Tensor qkv, at::Tensor cu_seqlens, int64_t max_seqlen, int64_t nq,
                                        int64_t nkv, double scale, bool want_lse, at::Tensor err, int64_t window,
                                           int64_t sinks) {
@@ -1147,7 +1174,10 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
                        const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k, int64_t max_q,
                        int64_t max_k, int64_t nq, int64_t nkv, int q_col, int k_col, int v_col, double scale,
                        at::Tensor& dq, int dq_col, at::Tensor& dkv, int dk_col, int dv_col, const at::Tensor& err,
-                       int64_t window, int64_t sinks) {
+                       int64_t window, int64_t sinks, const c10::optional<at::Tensor>& o_lo) {
+  if (o_lo.has_value())
+    TORCH_CHECK(o_lo->scalar_type() == at::kBFloat16 && o_lo->is_contiguous() && o_lo->numel() == o.numel(),
+                "o_lo must be contiguous bf16 like o");
   CHECK_DTYPE(q, at::kBFloat16);
   CHECK_DTYPE(kv, at::kBFloat16);
   CHECK_DTYPE(o, at::kBFloat16);
@@ -1164,8 +1194,9 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
   {
     const int64_t warps = T * nq;
     fa_bwd_dot<<<(unsigned)((warps * 32 + 255) / 256), 256, 0, stream()>>>(
-        reinterpret_cast<const bf16*>(o.data_ptr()), reinterpret_cast<const bf16*>(dout.data_ptr()), T, (int)nq,
-        dd.data_ptr<float>(), window > 0 ? cu_q.data_ptr<int>() + B : nullptr, reinterpret_cast<bf16*>(dq.data_ptr()),
+        reinterpret_cast<const bf16*>(o.data_ptr()),
+        o_lo.has_value() ? reinterpret_cast<const bf16*>(o_lo->data_ptr()) : nullptr,
+        reinterpret_cast<const bf16*>(dout.data_ptr()), T, (int)nq, dd.data_ptr<float>(), window > 0 ? cu_q.data_ptr<int>() + B : nullptr, reinterpret_cast<bf16*>(dq.data_ptr()),
         dq.stride(0), dq_col, same ? reinterpret_cast<bf16*>(dkv.data_ptr()) + dk_col : nullptr, dkv.stride(0),
         same ? (int)(2 * nkv * D) : 0);
     PSRL_CHECK_LAUNCH();
@@ -1237,7 +1268,7 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
 // [T, nq * 128] (bf16), lse [nq, T].  Returns dqkv [T, (nq + 2 nkv) * 128] bf16.
 at::Tensor attn_bwd_sm100(at::Tensor qkv, at::Tensor o, at::Tensor dout, at::Tensor lse, at::Tensor cu_seqlens,
                           int64_t max_seqlen, int64_t nq, int64_t nkv, double scale, at::Tensor err, int64_t window,
-                          int64_t sinks) {
+                          int64_t sinks, c10::optional<at::Tensor> o_lo) {
   CHECK_CUDA_TENSOR(qkv);
   TORCH_CHECK(qkv.dim() == 2 && qkv.size(1) == (nq + 2 * nkv) * D && nq % nkv == 0, "qkv layout");
   at::cuda::CUDAGuard g(qkv.device());
@@ -1245,7 +1276,7 @@ at::Tensor attn_bwd_sm100(at::Tensor qkv, at::Tensor o, at::Tensor dout, at::Ten
   if (qkv.size(0) == 0 || cu_seqlens.numel() < 2 || max_seqlen <= 0) return dqkv.zero_();
   const int kc = (int)(nq * D), vc = (int)((nq + nkv) * D);
   bwd_launch(qkv, qkv, o, dout, lse, cu_seqlens, cu_seqlens, max_seqlen, max_seqlen, nq, nkv, 0, kc, vc, scale, dqkv,
-             0, dqkv, kc, vc, err, window, sinks);
+             0, dqkv, kc, vc, err, window, sinks, o_lo);
   return dqkv;
 }
 
@@ -1253,7 +1284,8 @@ at::Tensor attn_bwd_sm100(at::Tensor qkv, at::Tensor o, at::Tensor dout, at::Ten
 // (bf16; key rows that no query sees get zero gradients).
 std::vector<at::Tensor> attn_bwd_sm100_kv(at::Tensor q, at::Tensor kv, at::Tensor o, at::Tensor dout, at::Tensor lse,
                                           at::Tensor cu_q, at::Tensor cu_k, int64_t max_q, int64_t max_k, int64_t nq,
-                                          int64_t nkv, double scale, at::Tensor err, int64_t window, int64_t sinks) {
+                                          int64_t nkv, double scale, at::Tensor err, int64_t window, int64_t sinks,
+                                          c10::optional<at::Tensor> o_lo) {
   CHECK_CUDA_TENSOR(q);
   TORCH_CHECK(q.dim() == 2 && q.size(1) >= nq * D && kv.dim() == 2 && kv.size(1) == 2 * nkv * D && nq % nkv == 0,
               "q [Tq, nq * 128], kv [Tk, 2 nkv * 128]");
@@ -1262,7 +1294,7 @@ std::vector<at::Tensor> attn_bwd_sm100_kv(at::Tensor q, at::Tensor kv, at::Tenso
   auto dkv = at::zeros({kv.size(0), 2 * nkv * D}, q.options());
   if (q.size(0) == 0 || cu_q.numel() < 2 || max_q <= 0) return {dq.zero_(), dkv};
   bwd_launch(q, kv, o, dout, lse, cu_q, cu_k, max_q, max_k, nq, nkv, 0, 0, (int)(nkv * D), scale, dq, 0, dkv, 0,
-             (int)(nkv * D), err, window, sinks);
+             (int)(nkv * D), err, window, sinks, o_lo);
   return {dq, dkv};
 }
 

@@ -68,13 +68,14 @@ std::vector<at::Tensor> attn_fwd_sm100_kv(at::Tensor q, at::Tensor kv, at::Tenso
                                           at::Tensor err, int64_t window, int64_t sinks);
 std::vector<at::Tensor> attn_bwd_sm100_kv(at::Tensor q, at::Tensor kv, at::Tensor o, at::Tensor dout, at::Tensor lse,
                                           at::Tensor cu_q, at::Tensor cu_k, int64_t max_q, int64_t max_k, int64_t nq,
-                                          int64_t nkv, double scale, at::Tensor err, int64_t window, int64_t sinks);
+                                          int64_t nkv, double scale, at::Tensor err, int64_t window, int64_t sinks,
+                                          c10::optional<at::Tensor> o_lo);
 std::vector<at::Tensor> attn_fwd_sm100(at::Tensor qkv, at::Tensor cu_seqlens, int64_t max_seqlen, int64_t nq,
                                        int64_t nkv, double scale, bool want_lse, at::Tensor err, int64_t window,
                                        int64_t sinks);
 at::Tensor attn_bwd_sm100(at::Tensor qkv, at::Tensor o, at::Tensor dout, at::Tensor lse, at::Tensor cu_seqlens,
                           int64_t max_seqlen, int64_t nq, int64_t nkv, double scale, at::Tensor err, int64_t window,
-                          int64_t sinks);
+                          int64_t sinks, c10::optional<at::Tensor> o_lo);
 std::vector<at::Tensor> moe_route(at::Tensor logits, c10::optional<at::Tensor> prior, int64_t k, bool renorm);
 std::vector<at::Tensor> moe_permute(at::Tensor ids, at::Tensor counts, int64_t bm, int64_t tiles_n);
 at::Tensor moe_gather(at::Tensor x, at::Tensor token_of_row);
@@ -142,10 +143,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("window") = 0, py::arg("sinks") = 0);
   m.def("attn_bwd_sm100_kv", &psrl::attn_bwd_sm100_kv, py::arg("q"), py::arg("kv"), py::arg("o"), py::arg("dout"),
         py::arg("lse"), py::arg("cu_q"), py::arg("cu_k"), py::arg("max_q"), py::arg("max_k"), py::arg("nq"),
-        py::arg("nkv"), py::arg("scale"), py::arg("err"), py::arg("window") = 0, py::arg("sinks") = 0);
+        py::arg("nkv"), py::arg("scale"), py::arg("err"), py::arg("window") = 0, py::arg("sinks") = 0,
+        py::arg("o_lo") = py::none());
   m.def("attn_bwd_sm100", &psrl::attn_bwd_sm100, py::arg("qkv"), py::arg("o"), py::arg("dout"), py::arg("lse"),
         py::arg("cu_seqlens"), py::arg("max_seqlen"), py::arg("nq"), py::arg("nkv"), py::arg("scale"), py::arg("err"),
-        py::arg("window") = 0, py::arg("sinks") = 0);
+        py::arg("window") = 0, py::arg("sinks") = 0, py::arg("o_lo") = py::none());
   m.def("moe_route", &psrl::moe_route);
   m.def("moe_permute", &psrl::moe_permute);
   m.def("moe_gather", &psrl::moe_gather);

@@ -124,23 +124,24 @@ class _VarlenAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, cu_seqlens, max_seqlen, nq, nkv, d, scale, window, sinks):
         T = qkv.shape[0]
-        o, lse = varlen_attention_fwd(qkv, cu_seqlens, max_seqlen, nq, nkv, scale, True, window, sinks)
+        # a windowed forward also returns what o's rounding left out (o_lo), for D = rowsum(do * o)
+        o, lse, o_lo = _varlen_fwd(qkv, cu_seqlens, max_seqlen, nq, nkv, scale, True, window, sinks)
         o = o.view(T, nq, d)
-        ctx.save_for_backward(qkv, o, lse, cu_seqlens)
+        ctx.save_for_backward(qkv, o, lse, cu_seqlens, o_lo)
         ctx.cfg = (max_seqlen, nq, nkv, d, scale, window, sinks)
         return o.view(T, nq * d)
 
     @staticmethod
     def backward(ctx, do):
         from .gemm import _err
-        qkv, o, lse, cu = ctx.saved_tensors
+        qkv, o, lse, cu, o_lo = ctx.saved_tensors
         max_seqlen, nq, nkv, d, scale, window, sinks = ctx.cfg
         if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
             qkv = qkv.contiguous()
         # tcgen05 backward (csrc/attn_sm100.cu): dK/dV per key tile and dQ per
         # query tile, written straight into one [T, (nq + 2 nkv) * d] gradient
         dqkv = ext().attn_bwd_sm100(qkv, o.reshape(qkv.shape[0], nq * d), do.contiguous(), lse, cu, max_seqlen,
-                                    nq, nkv, scale, _err(qkv.device), window, sinks)
+                                    nq, nkv, scale, _err(qkv.device), window, sinks, o_lo)
         return dqkv, None, None, None, None, None, None, None, None
 
 
@@ -149,6 +150,10 @@ def varlen_attention_fwd(qkv: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen
     """Forward of causal varlen attention on the tcgen05 kernel
     (``csrc/attn_sm100.cu``): ``qkv`` [T, (nq + 2 nkv) * 128] bf16 ->
     (o [T, nq * 128] bf16, lse [nq, T] fp32 natural log).  ``window`` 0: none."""
+    return tuple(_varlen_fwd(qkv, cu_seqlens, max_seqlen, nq, nkv, scale, want_lse, window, sinks)[:2])
+
+
+def _varlen_fwd(qkv, cu_seqlens, max_seqlen, nq, nkv, scale, want_lse, window, sinks):
     from .gemm import _err
     if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
         qkv = qkv.contiguous()
@@ -288,19 +293,19 @@ class _AttnKVFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, kv, cu_q, cu_k, max_q, max_k, nq, nkv, scale, window, sinks):
         from .gemm import _err
-        o, lse = ext().attn_fwd_sm100_kv(q, kv, cu_q, cu_k, int(max_q), int(nq), int(nkv), float(scale), True,
+        o, lse, o_lo = ext().attn_fwd_sm100_kv(q, kv, cu_q, cu_k, int(max_q), int(nq), int(nkv), float(scale), True,
                                          _err(q.device), window, sinks)
-        ctx.save_for_backward(q, kv, o, lse, cu_q, cu_k)
+        ctx.save_for_backward(q, kv, o, lse, cu_q, cu_k, o_lo)
         ctx.cfg = (max_q, max_k, nq, nkv, scale, window, sinks)
         return o
 
     @staticmethod
     def backward(ctx, do):
         from .gemm import _err
-        q, kv, o, lse, cu_q, cu_k = ctx.saved_tensors
+        q, kv, o, lse, cu_q, cu_k, o_lo = ctx.saved_tensors
         max_q, max_k, nq, nkv, scale, window, sinks = ctx.cfg
         dq, dkv = ext().attn_bwd_sm100_kv(q, kv, o, do.contiguous(), lse, cu_q, cu_k, int(max_q), int(max_k),
-                                          int(nq), int(nkv), float(scale), _err(q.device), window, sinks)
+                                          int(nq), int(nkv), float(scale), _err(q.device), window, sinks, o_lo)
         return dq, dkv, None, None, None, None, None, None, None, None, None
 
 
