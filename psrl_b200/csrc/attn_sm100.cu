@@ -424,7 +424,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 //                into TMEM) and accumulates dV += P^T dO_i and
 //                dK += dS^T Q_i in TMEM (A operands from TMEM, B read MN-major).
 //   fa_bwd_dq    one CTA per (query head, sequence, 128-row tile i): Q_i and
-//                dO_i stay in shared memory; for every key tile j <= i it
+//                dO_i stay in tensor memory as A operands (a 128 x 64 product
+//                whose A comes from shared memory is bound by fetching it:
+//                measured 1970 cycles a step against 1024); for every key tile j <= i it
 //                recomputes S = Q_i K_j^T and dP = dO_i V_j^T, forms dS and
 //                accumulates dQ += dS K_j.
 // D = rowsum(dO * O) comes from fa_bwd_dot.  Softmax work uses eight warps,
@@ -441,7 +443,7 @@ struct BwdArgs {
   int nq, nkv, T;
   int blocks_z;      // query tiles of the longest sequence (dQ grid)
   float scale, scale_log2;
-  const float* lse;  // [nq, T] natural log
+  const float* lse;  // [nq, T], base 2
   const float* dd;   // [nq, T] rowsum(dO * O)
   bf16* dq;          // query-gradient rows (dq_row apart), head 0 at column dq_col
   int64_t dq_row;
@@ -462,7 +464,8 @@ struct BwdArgs {
 // o_lo (or null): what o's rounding to bf16 left out; D is then as exact as P, dP
 // are (an error of D is common to a row's dS and does not average out over its keys)
 __global__ void fa_bwd_dot(const bf16* __restrict__ o, const bf16* __restrict__ o_lo, const bf16* __restrict__ dout, int64_t T, int nq,
-                           float* __restrict__ dd, const int* __restrict__ cu_end, bf16* __restrict__ dq,
+                           const float* __restrict__ lse, float* __restrict__ lse2, float* __restrict__ dd,
+                           const int* __restrict__ cu_end, bf16* __restrict__ dq,
                            int64_t dq_row, int dq_col, bf16* __restrict__ dkv, int64_t dkv_row, int dkv_cols) {
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
@@ -489,7 +492,10 @@ __global__ void fa_bwd_dot(const bf16* __restrict__ o, const bf16* __restrict__ 
     for (int i = 0; i < 4; ++i) s += __bfloat162float(pl[i]) * __bfloat162float(pd[i]);
   }
   s = warp_sum(s);
-  if (lane == 0) dd[(int64_t)h * T + t] = s;
+  if (lane == 0) {
+    dd[(int64_t)h * T + t] = s;
+    lse2[(int64_t)h * T + t] = lse[(int64_t)h * T + t] * 1.4426950408889634f;
+  }
 }
 
 // Adds the hsplit fp32 partial dK / dV rows of fa_bwd_dkdv and writes bf16
@@ -528,7 +534,7 @@ constexpr int ATOM64 = 64 * 64 * 2;          // 64 rows x 64 bf16 (one 128-byte 
 constexpr int KV64_TILE = 2 * ATOM64;        // 16 KB
 constexpr int NSQ = 4;                       // K/V ring depth of the dQ kernel
 constexpr int DQ_STAGE = 2 * KV64_TILE;      // K + V
-constexpr int OFF_DQ_KV = 2 * KV_TILE;       // after the resident Q and dO tiles
+constexpr int OFF_DQ_KV = 0;
 constexpr int OFF_DQ_BAR = OFF_DQ_KV + NSQ * DQ_STAGE;
 constexpr int SMEM_DQ = OFF_DQ_BAR + 256 + 1024;
 
@@ -567,7 +573,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OFF_DKV_BAR);
-  // kv_full, st_full[NSK] (count 2: TMA bytes + the lse/D copy), st_empty[NSK],
+  // kv_full, st_full[NSK] (count 33: TMA bytes + each producer lane's lse / D copies), st_empty[NSK],
   // s_full[2], p_full[2], done; then the TMEM slot
   const uint32_t bkv = smem_u32(bars), bsf0 = bkv + 8, bse0 = bsf0 + 8 * NSK, bs0 = bse0 + 8 * NSK, bp0 = bs0 + 16,
                  bdone = bp0 + 16;
@@ -578,7 +584,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
     s_abort = 0;
     mbar_init(bkv, 1);
     for (int k = 0; k < NSK; ++k) {
-      mbar_init(bsf0 + 8 * k, 2);
+      mbar_init(bsf0 + 8 * k, 33);
       mbar_init(bse0 + 8 * k, 1);
     }
     for (int k = 0; k < 2; ++k) {
@@ -636,17 +642,18 @@ __global__ void __launch_bounds__(NT_BWD, 1)
         tma_load_2d(sdo, &tm_do64, hq * D, y, fb);
         tma_load_2d(sdo + ATOM64, &tm_do64, hq * D + 64, y, fb);
       }
-      float* lse_s = reinterpret_cast<float*>(stg + 2 * KV64_TILE);
-      float* dd_s = lse_s + BQ2;
+      // lse and D of the 64 queries, asynchronously too: a producer that waited for
+      // plain loads here took 3200 cycles a step, the matrix products 1300
 #pragma unroll
-      for (int c = lane; c < BQ2; c += 32) {
-        const int q = i * BQ2 + c;
-        const bool in = q < L;
-        lse_s[c] = in ? a.lse[(int64_t)hq * a.T + s0 + q] * 1.4426950408889634f : 0.f;
-        dd_s[c] = in ? a.dd[(int64_t)hq * a.T + s0 + q] : 0.f;
+      for (int c = lane; c < 2 * BQ2; c += 32) {
+        const int q = i * BQ2 + (c & (BQ2 - 1));
+        const float* src = c < BQ2 ? a.lse : a.dd;
+        if (q < L) src += (int64_t)hq * a.T + s0 + q;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                     ::"r"(smem_u32(stg) + 2 * KV64_TILE + c * 4), "l"(src), "r"(q < L ? 4 : 0)
+                     : "memory");
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(fb);
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(fb) : "memory");
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -734,8 +741,8 @@ __global__ void __launch_bounds__(NT_BWD, 1)
       // no per-element mask
       const bool full = (i + 1) * BQ2 <= L && (j + 1) * BKV - 1 <= i * BQ2 + off &&
                         (!WIN || (i + 1) * BQ2 - 1 + off - j * BKV < a.window || (j + 1) * BKV <= a.sinks);
+      mbar_wait(bsf0 + 8 * st, (it / NSK) & 1);  // complete, as S^T of this step is: lse and D are there
       if (WIN && (i + 1) * BQ2 > L) {
-        mbar_wait(bsf0 + 8 * st, (it / NSK) & 1);  // complete: S^T of this step is
         uint8_t* stg = smem + OFF_DKV_STAGE + st * DKV_STAGE;
         zero_rows(stg, L - i * BQ2, BQ2, threadIdx.x - 64, 256);
         zero_rows(stg + KV64_TILE, L - i * BQ2, BQ2, threadIdx.x - 64, 256);
@@ -840,8 +847,8 @@ __global__ void __launch_bounds__(NT_BWD, 1)
 
 template <bool WIN>
 __global__ void __launch_bounds__(NT_BWD, 1)
-    fa_bwd_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV64,
-              const __grid_constant__ CUtensorMap tm_do, BwdArgs a) {
+    fa_bwd_dq(const __grid_constant__ CUtensorMap tmKV64, const bf16* __restrict__ qp, int64_t q_row,
+              const bf16* __restrict__ dop, BwdArgs a) {
   const int h = blockIdx.x, b = blockIdx.y;
   const int i = a.blocks_z - 1 - (int)blockIdx.z;  // large query tiles (most key tiles) first
   const int s0 = a.cu[b], L = a.cu[b + 1] - s0;
@@ -867,7 +874,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     s_abort = 0;
-    mbar_init(bqd, 1);
+    mbar_init(bqd, 8);  // one arrive per elementwise warp: Q and dO are in tensor memory
     for (int k = 0; k < NSQ; ++k) {
       mbar_init(bkf0 + 8 * k, 1);
       mbar_init(bke0 + 8 * k, 1);
@@ -884,23 +891,14 @@ __global__ void __launch_bounds__(NT_BWD, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
-  // TMEM columns: S_0 0..63, dP_0 64..127, S_1 128..191, dP_1 192..255, dQ 256..383
+  // TMEM columns: S_0 0..63, dP_0 64..127, S_1 128..191, dP_1 192..255, dQ 256..383, Q 384..447, dO 448..511
   auto tS = [&](int bb) { return tmem + 128u * (uint32_t)bb; };
   auto tP = [&](int bb) { return tmem + 128u * (uint32_t)bb + 64u; };
-  const uint32_t tdQ = tmem + 256;
-  const uint32_t sq = smem_u32(smem), sdo = sq + KV_TILE;
+  const uint32_t tdQ = tmem + 256, tQ = tmem + 384, tdO = tmem + 448;
 
   if (warp == 0) {
     if (lane == 0) {
-      tma_prefetch_desc(&tmQ);
       tma_prefetch_desc(&tmKV64);
-      tma_prefetch_desc(&tm_do);
-      mbar_expect_tx(bqd, 2 * KV_TILE);
-      const int y = s0 + i * BQ;
-      tma_load_2d(sq, &tmQ, a.q_col + h * D, y, bqd);
-      tma_load_2d(sq + ATOM, &tmQ, a.q_col + h * D + 64, y, bqd);
-      tma_load_2d(sdo, &tm_do, h * D, y, bqd);
-      tma_load_2d(sdo + ATOM, &tm_do, h * D + 64, y, bqd);
       for (int jj = 0; jj < n && !s_abort; ++jj) {
         const int st = jj % NSQ;
         const uint32_t ph = (jj / NSQ) & 1;
@@ -932,18 +930,19 @@ __global__ void __launch_bounds__(NT_BWD, 1)
         const int bb = jj & 1;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t oa = (k >> 2) * ATOM + (k & 3) * 32, ob = (k >> 2) * ATOM64 + (k & 3) * 32;
-          mma_1cta(tS(bb), desc_sw128(sq + oa, 16, 1024), desc_sw128(sk + ob, 16, 1024), id_s, k > 0);
+          const uint32_t ob = (k >> 2) * ATOM64 + (k & 3) * 32;
+          mma_1cta_ts(tS(bb), tQ + k * 8, desc_sw128(sk + ob, 16, 1024), id_s, k > 0);
         }
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t oa = (k >> 2) * ATOM + (k & 3) * 32, ob = (k >> 2) * ATOM64 + (k & 3) * 32;
-          mma_1cta(tP(bb), desc_sw128(sdo + oa, 16, 1024), desc_sw128(sv + ob, 16, 1024), id_s, k > 0);
+          const uint32_t ob = (k >> 2) * ATOM64 + (k & 3) * 32;
+          mma_1cta_ts(tP(bb), tdO + k * 8, desc_sw128(sv + ob, 16, 1024), id_s, k > 0);
         }
         commit_1cta(bs0 + 8 * bb);
         return true;
       };
       bool ok = mbar_wait(bqd, 0);
+      fence_after();
       int where = 0;
       if (ok && n > 0) {
         ok = issue_sdp(0);
@@ -986,7 +985,31 @@ __global__ void __launch_bounds__(NT_BWD, 1)
     const int q = i * BQ + r;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const bool qin = q < L;
-    const float lse2 = qin ? a.lse[(int64_t)h * a.T + s0 + q] * 1.4426950408889634f : 0.f;
+    {
+      // row r of Q (group 0) or dO (group 1) into tensor memory, two values per column;
+      // rows past the sequence are zeros
+      const bf16* src = half == 0 ? qp + (int64_t)(s0 + q) * q_row + a.q_col + h * D
+                                  : dop + ((int64_t)(s0 + q) * a.nq + h) * D;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t w[32];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (qin) x = *reinterpret_cast<const uint4*>(src + c * 64 + k * 8);
+          w[4 * k] = x.x;
+          w[4 * k + 1] = x.y;
+          w[4 * k + 2] = x.z;
+          w[4 * k + 3] = x.w;
+        }
+        tmem_st32((half == 0 ? tQ : tdO) + lane_off + c * 32, w);
+      }
+      tmem_wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bqd);
+    }
+    const float lse2 = qin ? a.lse[(int64_t)h * a.T + s0 + q] : 0.f;
     const float dd = qin ? a.dd[(int64_t)h * a.T + s0 + q] : 0.f;
     const int col0 = half * 32;
     bool ok = true;
@@ -1189,19 +1212,23 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
   TORCH_CHECK(lse.is_contiguous() && lse.numel() == nq * T, "lse must be contiguous [nq, Tq]");
   const int B = (int)cu_q.numel() - 1;
   if (T == 0 || B <= 0 || max_q <= 0) return;
-  auto dd = at::empty({nq, T}, q.options().dtype(at::kFloat));
+  auto dd = at::empty({nq, T}, q.options().dtype(at::kFloat)), lse2 = at::empty_like(dd);
   const bool same = dq.data_ptr() == dkv.data_ptr();  // one [q | k | v] gradient
   {
     const int64_t warps = T * nq;
     fa_bwd_dot<<<(unsigned)((warps * 32 + 255) / 256), 256, 0, stream()>>>(
         reinterpret_cast<const bf16*>(o.data_ptr()),
         o_lo.has_value() ? reinterpret_cast<const bf16*>(o_lo->data_ptr()) : nullptr,
-        reinterpret_cast<const bf16*>(dout.data_ptr()), T, (int)nq, dd.data_ptr<float>(), window > 0 ? cu_q.data_ptr<int>() + B : nullptr, reinterpret_cast<bf16*>(dq.data_ptr()),
+        reinterpret_cast<const bf16*>(dout.data_ptr()), T, (int)nq, lse.data_ptr<float>(), lse2.data_ptr<float>(),
+        dd.data_ptr<float>(), window > 0 ? cu_q.data_ptr<int>() + B : nullptr, reinterpret_cast<bf16*>(dq.data_ptr()),
         dq.stride(0), dq_col, same ? reinterpret_cast<bf16*>(dkv.data_ptr()) + dk_col : nullptr, dkv.stride(0),
         same ? (int)(2 * nkv * D) : 0);
     PSRL_CHECK_LAUNCH();
   }
-  const CUtensorMap tq = map_rows_64x128(q), tkv = map_rows_64x128(kv), tdo = map_rows_64x128(dout.view({T, nq * D}));
+  const CUtensorMap tkv = map_rows_64x128(kv);
+  TORCH_CHECK(q.stride(0) % 8 == 0 && q_col % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 == 0,
+              "query and output-gradient rows must start on 16-byte boundaries");
   BwdArgs a{};
   a.cu = cu_q.data_ptr<int>();
   a.cu_k = cu_k.data_ptr<int>();
@@ -1214,7 +1241,7 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
   a.blocks_z = (int)((max_q + BQ - 1) / BQ);
   a.scale = (float)scale;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
-  a.lse = lse.data_ptr<float>();
+  a.lse = lse2.data_ptr<float>();
   a.dd = dd.data_ptr<float>();
   a.dq = reinterpret_cast<bf16*>(dq.data_ptr());
   a.dq_row = dq.stride(0);
@@ -1260,7 +1287,8 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
     PSRL_CHECK_LAUNCH();
   }
   const CUtensorMap tkv64 = map_rows_64xR(kv, 64u);
-  kern_dq<<<dim3((unsigned)nq, (unsigned)B, (unsigned)a.blocks_z), NT_BWD, SMEM_DQ, stream()>>>(tq, tkv64, tdo, a);
+  kern_dq<<<dim3((unsigned)nq, (unsigned)B, (unsigned)a.blocks_z), NT_BWD, SMEM_DQ, stream()>>>(
+      tkv64, reinterpret_cast<const bf16*>(q.data_ptr()), q.stride(0), reinterpret_cast<const bf16*>(dout.data_ptr()), a);
   PSRL_CHECK_LAUNCH();
 }
 
