@@ -257,22 +257,25 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (j > v_ready) ok = ok && mbar_wait(bvf + 8 * (j & 1), (j >> 1) & 1);
         v_ready = j;
       };
+      // descriptors: a base per operand, constants added per product
+      constexpr uint64_t T16 = TILE >> 4;
+      const uint64_t dQ = desc_sw128(smem_u32(smem), 16, 1024), dK = desc_sw128(smem_u32(smem + OFF_K), 16, 1024);
+      const uint64_t dV = desc_sw128(smem_u32(smem + OFF_V), ATOM, 1024);
       auto issue_s = [&](int g, int j) {
         fence_after();
-        const uint32_t sq = smem_u32(smem + g * TILE), sk = smem_u32(smem + OFF_K + (j & 1) * TILE);
+        const uint64_t q = dQ + g * T16, kk = dK + (j & 1) * T16;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t o = (k >> 2) * ATOM + (k & 3) * 32;
-          mma_1cta(tS(g), desc_sw128(sq + o, 16, 1024), desc_sw128(sk + o, 16, 1024), idesc_qk, k > 0);
+          const uint64_t o = ((k >> 2) * ATOM + (k & 3) * 32) >> 4;
+          mma_1cta(tS(g), q + o, kk + o, idesc_qk, k > 0);
         }
         commit_1cta(bsf + 8 * g);
       };
       auto issue_pv = [&](int g, int j) {
         fence_after();
-        const uint32_t sv = smem_u32(smem + OFF_V + (j & 1) * TILE);
+        const uint64_t v = dV + (j & 1) * T16;
 #pragma unroll
-        for (int k = 0; k < BKV / 16; ++k)
-          mma_1cta_ts(tO(g), tS(g) + k * 8, desc_sw128(sv + k * 2048, ATOM, 1024), idesc_pv, (j > 0 || k > 0));
+        for (int k = 0; k < BKV / 16; ++k) mma_1cta_ts(tO(g), tS(g) + k * 8, v + (k * 2048 >> 4), idesc_pv, (j > 0 || k > 0));
       };
       if (nK > 0 && ok) {
         wait_k(0);

@@ -79,6 +79,13 @@ struct FwdArgs {
   int* err;
 };
 
+// Descriptor steps in 16-byte units: the MMA thread adds one of these constants to
+// a base it keeps per operand.  (Composing a descriptor per MMA cost that single
+// thread about 100 cycles each, more than the product itself.)
+__host__ __device__ constexpr uint64_t step_k(int k, int atom) { return (uint64_t)(((k >> 2) * atom + (k & 3) * 32) >> 4); }
+__host__ __device__ constexpr uint64_t step_mn(int k) { return (uint64_t)(k * 2048 >> 4); }
+constexpr uint64_t units(int bytes) { return (uint64_t)(bytes >> 4); }
+
 // First failure of the launch: code, then (block x, y, z, warp, iteration) in err[1..5].
 __device__ __forceinline__ void set_err(int* err, int code, int it = -1) {
   if (err && atomicCAS(err, 0, code) == 0) {
@@ -216,22 +223,20 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
         kv_ready = j;
       };
+      const uint64_t dQ = desc_sw128(smem_u32(smem), 16, 1024), dK = desc_sw128(smem_u32(smem + OFF_KV), 16, 1024);
+      const uint64_t dV = desc_sw128(smem_u32(smem + OFF_KV + KV_TILE), ATOM, 1024);
       auto issue_s = [&](int g, int j) {
         fence_after();
-        const uint32_t sq = smem_u32(smem + g * Q_BYTES), sk = smem_u32(smem + OFF_KV + (j % NS) * STAGE);
+        const uint64_t q = dQ + g * units(Q_BYTES), kk = dK + (j % NS) * units(STAGE);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * ATOM + (k & 3) * 32;
-          mma_1cta(tS(g), desc_sw128(sq + off, 16, 1024), desc_sw128(sk + off, 16, 1024), idesc_qk, k > 0);
-        }
+        for (int k = 0; k < D / 16; ++k) mma_1cta(tS(g), q + step_k(k, ATOM), kk + step_k(k, ATOM), idesc_qk, k > 0);
         commit_1cta(bsf + 8 * g);
       };
       auto issue_pv = [&](int g, int j, bool first) {
         fence_after();
-        const uint32_t sv = smem_u32(smem + OFF_KV + (j % NS) * STAGE + KV_TILE);
+        const uint64_t v = dV + (j % NS) * units(STAGE);
 #pragma unroll
-        for (int k = 0; k < BKV / 16; ++k)
-          mma_1cta_ts(tO(g), tS(g) + k * 8, desc_sw128(sv + k * 2048, ATOM, 1024), idesc_pv, (!first || k > 0));
+        for (int k = 0; k < BKV / 16; ++k) mma_1cta_ts(tO(g), tS(g) + k * 8, v + step_mn(k), idesc_pv, (!first || k > 0));
       };
       wait_kv(0);
       if (ok) {
@@ -659,24 +664,22 @@ __global__ void __launch_bounds__(NT_BWD, 1)
     if (lane == 0) {
       constexpr uint32_t id_ss = idesc_bf16_f32(BKV, BQ2, false, false);  // M = keys, N = 64 queries
       constexpr uint32_t id_ts = idesc_bf16_f32(BKV, D, false, true);     // M = keys, N = d, K = 64 queries
-      const uint32_t sk = smem_u32(smem), sv = sk + KV_TILE;
+      const uint64_t dK = desc_sw128(smem_u32(smem), 16, 1024), dV = desc_sw128(smem_u32(smem) + KV_TILE, 16, 1024);
+      // Q and dO of a stage, K-major (S^T, dP^T) and MN-major (dK, dV)
+      const uint32_t st0 = smem_u32(smem + OFF_DKV_STAGE);
+      const uint64_t dQ = desc_sw128(st0, 16, 1024), dO = desc_sw128(st0 + KV64_TILE, 16, 1024);
+      const uint64_t dQt = desc_sw128(st0, ATOM64, 1024), dOt = desc_sw128(st0 + KV64_TILE, ATOM64, 1024);
       // S^T = K Q^T and dP^T = V dO^T of step it into buffer it & 1
       auto issue_s = [&](int it) -> bool {
         const int st = it % NSK;
         if (!mbar_wait(bsf0 + 8 * st, (it / NSK) & 1)) return false;
         fence_after();
-        const uint32_t sq = smem_u32(smem + OFF_DKV_STAGE + st * DKV_STAGE), sdo = sq + KV64_TILE;
+        const uint64_t q = dQ + st * units(DKV_STAGE), dd = dO + st * units(DKV_STAGE);
         const int bb = it & 1;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t oa = (k >> 2) * ATOM + (k & 3) * 32, ob = (k >> 2) * ATOM64 + (k & 3) * 32;
-          mma_1cta(tS(bb), desc_sw128(sk + oa, 16, 1024), desc_sw128(sq + ob, 16, 1024), id_ss, k > 0);
-        }
+        for (int k = 0; k < D / 16; ++k) mma_1cta(tS(bb), dK + step_k(k, ATOM), q + step_k(k, ATOM64), id_ss, k > 0);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t oa = (k >> 2) * ATOM + (k & 3) * 32, ob = (k >> 2) * ATOM64 + (k & 3) * 32;
-          mma_1cta(tP(bb), desc_sw128(sv + oa, 16, 1024), desc_sw128(sdo + ob, 16, 1024), id_ss, k > 0);
-        }
+        for (int k = 0; k < D / 16; ++k) mma_1cta(tP(bb), dV + step_k(k, ATOM), dd + step_k(k, ATOM64), id_ss, k > 0);
         commit_1cta(bs0 + 8 * bb);
         return true;
       };
@@ -702,14 +705,14 @@ __global__ void __launch_bounds__(NT_BWD, 1)
         }
         fence_after();
         const int st = it % NSK;
-        const uint32_t sq = smem_u32(smem + OFF_DKV_STAGE + st * DKV_STAGE), sdo = sq + KV64_TILE;
+        const uint64_t q = dQt + st * units(DKV_STAGE), dd = dOt + st * units(DKV_STAGE);
         // P^T and dS^T (bf16) sit packed in columns [0, 16) and [32, 48) of S^T_bb and dP^T_bb
 #pragma unroll
         for (int k = 0; k < BQ2 / 16; ++k) {
           const uint32_t acol = (k < 2) ? k * 8 : 32 + (k - 2) * 8;
           const uint32_t acc = (it > 0 || k > 0) ? 1u : 0u;
-          mma_1cta_ts(tdV, tS(bb) + acol, desc_sw128(sdo + k * 2048, ATOM64, 1024), id_ts, acc);  // dV += P^T dO
-          mma_1cta_ts(tdK, tP(bb) + acol, desc_sw128(sq + k * 2048, ATOM64, 1024), id_ts, acc);   // dK += dS^T Q
+          mma_1cta_ts(tdV, tS(bb) + acol, dd + step_mn(k), id_ts, acc);  // dV += P^T dO
+          mma_1cta_ts(tdK, tP(bb) + acol, q + step_mn(k), id_ts, acc);   // dK += dS^T Q
         }
         commit_1cta(bse0 + 8 * st);  // Q / dO of this step no longer read
       }
@@ -921,23 +924,20 @@ __global__ void __launch_bounds__(NT_BWD, 1)
     if (lane == 0) {
       constexpr uint32_t id_s = idesc_bf16_f32(BQ, BK2, false, false);  // M = queries, N = 64 keys
       constexpr uint32_t id_dq = idesc_bf16_f32(BQ, D, false, true);    // M = queries, N = d, K = 64 keys
+      const uint32_t kv0 = smem_u32(smem + OFF_DQ_KV);
+      const uint64_t dK = desc_sw128(kv0, 16, 1024), dV = desc_sw128(kv0 + KV64_TILE, 16, 1024);
+      const uint64_t dKt = desc_sw128(kv0, ATOM64, 1024);
       // S = Q K^T and dP = dO V^T of key tile jj into buffer jj & 1
       auto issue_sdp = [&](int jj) -> bool {
         const int st = jj % NSQ;
         if (!mbar_wait(bkf0 + 8 * st, (jj / NSQ) & 1)) return false;
         fence_after();
-        const uint32_t sk = smem_u32(smem + OFF_DQ_KV + st * DQ_STAGE), sv = sk + KV64_TILE;
+        const uint64_t kk = dK + st * units(DQ_STAGE), v = dV + st * units(DQ_STAGE);
         const int bb = jj & 1;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t ob = (k >> 2) * ATOM64 + (k & 3) * 32;
-          mma_1cta_ts(tS(bb), tQ + k * 8, desc_sw128(sk + ob, 16, 1024), id_s, k > 0);
-        }
+        for (int k = 0; k < D / 16; ++k) mma_1cta_ts(tS(bb), tQ + k * 8, kk + step_k(k, ATOM64), id_s, k > 0);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t ob = (k >> 2) * ATOM64 + (k & 3) * 32;
-          mma_1cta_ts(tP(bb), tdO + k * 8, desc_sw128(sv + ob, 16, 1024), id_s, k > 0);
-        }
+        for (int k = 0; k < D / 16; ++k) mma_1cta_ts(tP(bb), tdO + k * 8, v + step_k(k, ATOM64), id_s, k > 0);
         commit_1cta(bs0 + 8 * bb);
         return true;
       };
@@ -963,12 +963,12 @@ __global__ void __launch_bounds__(NT_BWD, 1)
           break;
         }
         fence_after();
-        const uint32_t sk = smem_u32(smem + OFF_DQ_KV + (jj % NSQ) * DQ_STAGE);
+        const uint64_t kk = dKt + (jj % NSQ) * units(DQ_STAGE);
         // dQ += dS K: dS (bf16) sits packed in columns [0, 16) and [32, 48) of S_bb
 #pragma unroll
         for (int k = 0; k < BK2 / 16; ++k) {
           const uint32_t acol = (k < 2) ? k * 8 : 32 + (k - 2) * 8;
-          mma_1cta_ts(tdQ, tS(bb) + acol, desc_sw128(sk + k * 2048, ATOM64, 1024), id_dq, (jj > 0 || k > 0) ? 1u : 0u);
+          mma_1cta_ts(tdQ, tS(bb) + acol, kk + step_mn(k), id_dq, (jj > 0 || k > 0) ? 1u : 0u);
         }
         commit_1cta(bke0 + 8 * (jj % NSQ));  // K_jj / V_jj no longer read
       }
