@@ -18,10 +18,12 @@
 //                   their exponent bytes, into a ring of raw half tiles
 //      warp 1       MMA issuer
 //      warps 4..11  softmax, one thread per row, tiles A and B
-//      warps 12..15 8-bit cache: codes to bf16, exactly (bits moved into place, times
-//                   a power of two), from the raw ring into the MMA's tiles
+//      warps 12..19 8-bit cache: codes to bf16, exactly (bits moved into place, times
+//                   a power of two), from the raw ring into the MMA's tiles; four
+//                   warps for K, four for V, so that neither waits for the other's
+//                   tile to become free
 //    Values at or past len count as zeros, whatever their page holds.
-//    Registers are moved from the first and last warpgroup to the softmax.
+//    With an 8-bit cache, registers are moved from the other warpgroups to the softmax.
 //  * Few query tiles: the key tiles of a block are split over CTAs, whose partial
 //    rows (fp32, with a base-2 log-sum) a second kernel joins in key order.
 //  * A vector with exponent 255 reads as NaN.  A value vector's NaN is carried by
@@ -51,7 +53,7 @@ constexpr int RK = BKV / 2, RAW = RK * D, NRAW = 4;
 constexpr int OFF_RAW = OFF_BAR + 256, OFF_EXP = OFF_RAW + NRAW * RAW;
 constexpr int smem_bytes(bool fp8) { return (fp8 ? OFF_EXP + NRAW * 2 * RK : OFF_BAR + 256) + 1024; }
 static_assert(smem_bytes(true) <= 227 * 1024, "shared memory of a block");
-constexpr int NTHREADS = 512;
+constexpr int threads_of(bool fp8) { return fp8 ? 640 : 384; }
 constexpr float RESCALE_LOG2 = 8.0f;
 
 struct Args {
@@ -103,9 +105,10 @@ __device__ __forceinline__ void bf16_of4(uint32_t w, uint32_t m, uint32_t* out) 
 }
 
 template <bool FP8>
-__global__ void __launch_bounds__(NTHREADS, 1)
+__global__ void __launch_bounds__(threads_of(FP8), 1)
     chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, Args a) {
+  constexpr int NTHREADS = threads_of(FP8);
   const int hk = blockIdx.x, b = blockIdx.y;
   const int blk = a.blocks_z - 1 - (int)blockIdx.z / a.splits, part = (int)blockIdx.z % a.splits;
   const int s0 = max(0, min(a.cu_q[b], a.T)), n = min(a.cu_q[b + 1], a.T) - s0;
@@ -177,7 +180,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   auto tO = [&](int g) { return tmem + 256u + 128u * (uint32_t)g; };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 0 && nK > 0) {
       // ----------------------------------------------------------- producer
       if (lane == 0) {
@@ -312,23 +315,23 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
   } else if (warp >= 12) {
     // ------------------------------------------------- codes to bf16 tiles
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     if constexpr (FP8) {
-      // a thread converts codes 16c.. of rows sub + 16 i of a half
-      const int ct = threadIdx.x - 384, sub = ct >> 3, c = ct & 7;
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+      // warps 12..15 convert K, 16..19 V; a thread codes 16c.. of rows sub + 16 i of a half
+      const bool is_v = warp >= 16;
+      const int ct = (threadIdx.x - 384) & 127, sub = ct >> 3, c = ct & 7;
       // the two 16-byte halves in an order that spreads a row's threads over all banks
       const int first = c >> 2, c0 = 2 * (c & 3);
       const int to0 = sub * 128 + (((c0 + first) ^ (sub & 7)) << 4), to1 = sub * 128 + (((c0 + 1 - first) ^ (sub & 7)) << 4);
       // RARE: an exponent that does not fit one bf16 factor (values of 2^16 and more), or keys past len
       auto convert = [&](auto rare, int h) {
         constexpr bool RARE = decltype(rare)::value;
-        const bool is_v = h & 2;
         const int j = h >> 2, st = h % NRAW;
         const uint8_t* from = smem + OFF_RAW + st * RAW + sub * D + c * 16;
         const uint8_t* ex = smem + OFF_EXP + st * 2 * RK + sub;
         uint8_t* tile = smem + (is_v ? OFF_V : OFF_K) + (j & 1) * TILE + (c >> 2) * ATOM + (h & 1) * RK * 128;
         const int left = len - key_tile(j) * BKV - (h & 1) * RK;  // rows of the half below len
-#pragma unroll
+#pragma unroll 2
         for (int i = 0; i < 4; ++i) {
           uint4 w = *reinterpret_cast<const uint4*>(from + i * 16 * D);
           if (RARE && i * 16 + sub >= left) w = make_uint4(0, 0, 0, 0);
@@ -356,9 +359,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
       };
       bool ok = true;
-      for (int h = 0; h < 4 * nK; ++h) {
+      for (int n2 = 0; n2 < 2 * nK; ++n2) {
+        const int h = 4 * (n2 >> 1) + (is_v ? 2 : 0) + (n2 & 1);
         const int j = h >> 2, st = h % NRAW;
-        const bool is_v = h & 2;
         ok = mbar_wait(brf + 8 * st, (h / NRAW) & 1);
         if (j >= 2 && !(h & 1)) ok = ok && mbar_wait((is_v ? bve : bke) + 8 * (j & 1), ((j >> 1) & 1) ^ 1);
         if (!__all_sync(0xffffffffu, ok) || s_abort) {
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
   } else {
     // -------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int g = (warp - 4) >> 2;  // 0: tile A (warps 4..7), 1: tile B (warps 8..11)
     const int nt = g == 0 ? nA : nB;
     const int quad = warp & 3;
@@ -649,7 +652,7 @@ at::Tensor attn_paged_chunk(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache
   const CUtensorMap tv = fp8 ? kv8::map_codes(v_cache, RK, CU_TENSOR_MAP_SWIZZLE_NONE) : map_pages(v_cache);
   auto* kern = fp8 ? chunk_kernel<true> : chunk_kernel<false>;
   ensure_smem_attr(kern, smem_bytes(fp8));
-  kern<<<dim3((unsigned)nkv, (unsigned)B, (unsigned)(a.blocks_z * splits)), NTHREADS, smem_bytes(fp8), stream()>>>(tq, tk, tv,
+  kern<<<dim3((unsigned)nkv, (unsigned)B, (unsigned)(a.blocks_z * splits)), threads_of(fp8), smem_bytes(fp8), stream()>>>(tq, tk, tv,
                                                                                                                         a);
   PSRL_CHECK_LAUNCH();
   if (splits > 1) {
