@@ -66,6 +66,7 @@ struct Args {
   int T, nq, nkv, group, tok;  // tok: tokens per query tile
   int max_blocks, block_shift;
   int window, sinks, splits, blocks_z;
+  int B, sms;
   float scale_log2;
   bf16* o;          // [T, nq, D]
   float* part_o;    // [splits][T][nq][D]
@@ -131,11 +132,43 @@ __global__ void __launch_bounds__(threads_of(FP8), 1)
   auto entries = [&](int last) { return last + off < 0 ? 0 : (last + off) / BKV + 1 - gap; };
   const int lA = entries(min(iB, n) - 1), lB = iB < n ? entries(iE - 1) : 0;
   const int all = max(lA, lB);
-  // this part's share, at least two tiles
-  const int per = max(2, (all + a.splits - 1) / a.splits);
+  // This part's share.  The parts of all blocks are equally long (at least two tiles), so that
+  // together they are about one per SM whatever the lengths; a block has as many as it needs
+  int per = all;
+  __shared__ int s_tiles, s_blocks;
+  if (a.splits > 1) {
+    if (threadIdx.x == 0) s_tiles = s_blocks = 0;
+    __syncthreads();
+    int tiles = 0, blocks = 0;
+    for (int i = threadIdx.x; i < a.B; i += NTHREADS) {
+      const int ni = max(0, min(a.cu_q[i + 1], a.T) - max(0, min(a.cu_q[i], a.T)));
+      const int li = max(0, min(a.kv_lens[i], a.max_blocks << a.block_shift));
+      const int nb = (ni + 2 * a.tok - 1) / (2 * a.tok);
+      int t = (li + BKV - 1) / BKV;
+      if (a.window > 0) t = min(t, (min(a.window, 1 << 24) + min(a.sinks, 1 << 24) + 2 * a.tok + BKV - 1) / BKV + 1);
+      tiles += nb * t;
+      blocks += nb;
+    }
+    if (tiles) {
+      atomicAdd(&s_tiles, tiles);
+      atomicAdd(&s_blocks, blocks);
+    }
+    __syncthreads();
+    const int spare = a.sms / a.nkv - s_blocks;
+    if (spare > 0) per = (s_tiles + spare - 1) / spare;
+    per = max(max(2, per), (all + a.splits - 1) / a.splits);
+  }
   const int j0 = part * per, j1 = min(all, j0 + per);
   const int nA = max(0, min(lA, j1) - j0), nB = max(0, min(lB, j1) - j0), nK = max(nA, nB);
   auto key_tile = [&](int j) { return j + j0 < ns ? j + j0 : j + j0 + gap; };
+  kv8::launch_dependents();
+  if (part > 0 && nK == 0) {
+    // nothing left for this part: its rows count for nothing in the join
+    for (int i = threadIdx.x; i < (iE - i0) * a.group; i += NTHREADS)
+      a.part_lse[(int64_t)part * a.T * a.nq + (int64_t)(s0 + i0 + i / a.group) * a.nq + hk * a.group + i % a.group] =
+          -INFINITY;
+    return;
+  }
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -527,6 +560,7 @@ __global__ void __launch_bounds__(256) chunk_join(Args a, int B) {
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   const int64_t rows = (int64_t)max(0, min(a.cu_q[B], a.T)) * a.nq;
+  kv8::wait_prior();  // every block: this kernel must not end before the one it follows
   if (w >= rows) return;
   const int64_t stride = (int64_t)a.T * a.nq;
   float m = -INFINITY;
@@ -633,12 +667,17 @@ at::Tensor attn_paged_chunk(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache
   a.err = err.data_ptr<int>();
   const int64_t per_block = 2 * a.tok;
   a.blocks_z = (int)((std::min(max_q_len, T) + per_block - 1) / per_block);
-  // Split the keys while the CTAs all fit on the SMs at once: CTAs with work are at
-  // most one per block of tokens; a part keeps four key tiles of the longest context.
+  // Split the keys while there are fewer blocks (at most one CTA each) than SMs.  How
+  // long a part is, the kernel finds from the lengths; here only the most parts that
+  // a block may get: four times its share of the SMs, none under two key tiles.
   const int64_t ctas = nkv * std::min<int64_t>(B * a.blocks_z, T / per_block + B);
   const int64_t span = window > 0 ? std::min(cap, window + a.sinks + per_block) : cap;
-  int64_t splits = std::min<int64_t>(num_sms() / ctas, (span + 4 * BKV - 1) / (4 * BKV));
-  splits = std::max<int64_t>(1, std::min<int64_t>(splits, 64));
+  int64_t splits = 1;
+  if (2 * ctas <= num_sms())
+    splits = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(4 * num_sms() / ctas, 64),
+                                                    (span + 2 * BKV - 1) / (2 * BKV)));
+  a.B = (int)B;
+  a.sms = num_sms();
   TORCH_CHECK(a.blocks_z * splits < 65536, "too many query blocks");
   a.splits = (int)splits;
   at::Tensor part;
@@ -656,8 +695,7 @@ at::Tensor attn_paged_chunk(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache
                                                                                                                         a);
   PSRL_CHECK_LAUNCH();
   if (splits > 1) {
-    chunk_join<<<(unsigned)((T * nq * 32 + 255) / 256), 256, 0, stream()>>>(a, (int)B);
-    PSRL_CHECK_LAUNCH();
+    kv8::launch_after(chunk_join, (unsigned)((T * nq * 32 + 255) / 256), 256u, a, (int)B);
   }
   return o;
 }

@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(NTHREADS, resident(NT))
   const int64_t total = scan_items<NTHREADS>(a, s_scan, &before, &blo, &bhi);
   const int64_t per = share_of(total, a.workers);
   const int64_t start = (int64_t)blockIdx.x * per, stop = min(total, start + per);
+  kv8::launch_dependents();
   if (start >= total) return;  // uniform
   for (int b = blo; b < bhi; ++b) {
     const int64_t n = (int64_t)tiles_of(a, b).n * a.nkv;
@@ -515,6 +516,7 @@ __global__ void __launch_bounds__(128) decode8_join(Args a) {
   __syncthreads();
   const int64_t per = share_of(total, a.workers);
   const int n = tiles_of(a, b).n;
+  kv8::wait_prior();  // every block: this kernel must not end before the one it follows
   bf16* out = a.o + ((int64_t)b * a.nq + h) * D;
   if (n == 0) {
     out[threadIdx.x] = __float2bfloat16(0.f);
@@ -620,8 +622,7 @@ at::Tensor attn_decode_fp8(at::Tensor q, at::Tensor k_cache, at::Tensor v_cache,
   ensure_smem_attr(kern, smem_bytes(nt));
   kern<<<a.workers, NTHREADS, smem_bytes(nt), stream()>>>(tk, tv, a);
   PSRL_CHECK_LAUNCH();
-  decode8_join<<<(unsigned)(B * nq), 128, 0, stream()>>>(a);
-  PSRL_CHECK_LAUNCH();
+  kv8::launch_after(decode8_join, (unsigned)(B * nq), 128u, a);
   return o;
 }
 

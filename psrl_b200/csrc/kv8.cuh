@@ -24,6 +24,25 @@ __device__ __forceinline__ uint32_t f16_of2_hi(uint32_t codes) {
   return r;
 }
 
+// Programmatic dependent launch: the joining kernel is put on the SMs while the
+// kernel before it still runs (launch_dependents there), computes what needs no
+// partials, and waits for that kernel's end and its writes (wait_prior).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void wait_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+inline void launch_after(void (*kern)(P...), unsigned grid, unsigned block, A... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(block);
+  c.stream = stream();
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  PSRL_CHECK_CUDA(cudaLaunchKernelEx(&c, kern, static_cast<P>(args)...));
+}
+
 // Tensor map over the codes: rows of 128 bytes (one vector each), boxes of
 // min(tile, block_size) rows.
 inline CUtensorMap map_codes(const at::Tensor& t, int tile, CUtensorMapSwizzle swizzle) {

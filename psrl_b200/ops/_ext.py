@@ -15,7 +15,7 @@ _ERR: Exception | None = None
 # Kernel launches issued through this module (host-side count).  CUDA-graph
 # replays are added by the engine from the count recorded at capture time.
 LAUNCHES = 0
-_KERNELS_PER_CALL = {"rmsnorm_bwd": 1, "sqnorm_accumulate_": 2, "attn_varlen_bwd": 2, "attn_decode_fp8": 2}
+_KERNELS_PER_CALL = {"rmsnorm_bwd": 1, "sqnorm_accumulate_": 2, "attn_varlen_bwd": 2, "attn_decode_fp8": 2, "attn_paged_chunk": 1}
 
 
 class _Counted:
@@ -38,6 +38,7 @@ class _Counted:
             LAUNCHES += n
             return fn(*a, **k)
 
+        self.__dict__[name] = wrapped      # found directly from now on
         return wrapped
 
 

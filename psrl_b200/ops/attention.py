@@ -16,6 +16,7 @@ import math
 import torch
 
 from ._ext import ext
+from .gemm import _err
 
 
 # --------------------------------------------------------------- references
@@ -133,7 +134,6 @@ class _VarlenAttnFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do):
-        from .gemm import _err
         qkv, o, lse, cu, o_lo = ctx.saved_tensors
         max_seqlen, nq, nkv, d, scale, window, sinks = ctx.cfg
         if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
@@ -154,7 +154,6 @@ def varlen_attention_fwd(qkv: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen
 
 
 def _varlen_fwd(qkv, cu_seqlens, max_seqlen, nq, nkv, scale, want_lse, window, sinks):
-    from .gemm import _err
     if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
         qkv = qkv.contiguous()
     return ext().attn_fwd_sm100(qkv, cu_seqlens, int(max_seqlen), int(nq), int(nkv), float(scale), bool(want_lse),
@@ -220,7 +219,6 @@ def paged_prefill_attention(q, k_cache, v_cache, cu_q, kv_lens, block_table, max
     if q.is_cuda and d == 128:
         if k_scale is None and not win:
             return ext().attn_paged_prefill(q, k_cache, v_cache, cu_q, kv_lens, block_table, int(max_q_len), scale)
-        from .gemm import _err
         if not (q.stride(2) == 1 and q.stride(1) % 8 == 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0):
             q = q.contiguous()
         return ext().attn_paged_chunk(q, k_cache, v_cache, k_scale, v_scale, cu_q, kv_lens, block_table,
@@ -249,8 +247,7 @@ def paged_decode_attention(q, k_cache, v_cache, block_table, kv_lens, scale=None
         if not (q.stride(2) == 1 and q.stride(1) == d and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0):
             q = q.contiguous()
         if k_scale is not None:
-            from .gemm import _err
-            return ext().attn_decode_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, kv_lens, scale, win,
+                return ext().attn_decode_fp8(q, k_cache, v_cache, k_scale, v_scale, block_table, kv_lens, scale, win,
                                          sinks, _err(q.device))
         if splits is None:
             ctx = int(block_table.shape[1] * k_cache.shape[2])
@@ -292,7 +289,6 @@ class _AttnKVFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, kv, cu_q, cu_k, max_q, max_k, nq, nkv, scale, window, sinks):
-        from .gemm import _err
         o, lse, o_lo = ext().attn_fwd_sm100_kv(q, kv, cu_q, cu_k, int(max_q), int(nq), int(nkv), float(scale), True,
                                          _err(q.device), window, sinks)
         ctx.save_for_backward(q, kv, o, lse, cu_q, cu_k, o_lo)
@@ -301,7 +297,6 @@ class _AttnKVFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do):
-        from .gemm import _err
         q, kv, o, lse, cu_q, cu_k, o_lo = ctx.saved_tensors
         max_q, max_k, nq, nkv, scale, window, sinks = ctx.cfg
         dq, dkv = ext().attn_bwd_sm100_kv(q, kv, o, do.contiguous(), lse, cu_q, cu_k, int(max_q), int(max_k),

@@ -25,6 +25,11 @@ from ._ext import ext
 from .rope import apply_rope_ref, rope_tables
 
 FP8 = torch.float8_e4m3fn
+_ROPE: dict = {}          # (theta, d, device) -> rotary tables, as rope_tables keeps them
+
+
+def _i32(x: torch.Tensor) -> torch.Tensor:
+    return x if x.dtype == torch.int32 else x.int()
 
 
 # --------------------------------------------------------------- references
@@ -71,11 +76,14 @@ def rope_quant_kv(qkv: torch.Tensor, positions: torch.Tensor, nq: int, nkv: int,
     ``positions`` [T] lie below the 65536 rows of the rotary table; a position
     outside it turns the token's queries and keys into NaN."""
     if qkv.is_cuda:
-        cos, sin = rope_tables(theta, d, 65536, qkv.device)
+        tabs = _ROPE.get((theta, d, qkv.device))
+        if tabs is None:
+            tabs = _ROPE[(theta, d, qkv.device)] = rope_tables(theta, d, 65536, qkv.device)
+        cos, sin = tabs
         if qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16:
             qkv = qkv.contiguous()
-        return ext().rope_quant_kv(qkv, positions.int(), cos, sin, int(nq), int(nkv), int(d), k_cache, v_cache,
-                                   k_scale, v_scale, slots.int())
+        return ext().rope_quant_kv(qkv, _i32(positions), cos, sin, int(nq), int(nkv), int(d), k_cache, v_cache,
+                                   k_scale, v_scale, _i32(slots))
     T = qkv.shape[0]
     if T == 0:
         return qkv.new_empty(0, nq * d)
@@ -96,7 +104,7 @@ def read_kv_cache(cache: torch.Tensor, scale: torch.Tensor, blocks: torch.Tensor
             raise ValueError("out_blocks name pages of out")
         out = torch.empty((blocks.numel(),) + tuple(cache.shape[1:]), dtype=torch.bfloat16, device=cache.device)
     if cache.is_cuda:
-        ext().read_kv_cache(cache, scale, blocks.int(), out, out_blocks.int() if out_blocks is not None else None)
+        ext().read_kv_cache(cache, scale, _i32(blocks), out, _i32(out_blocks) if out_blocks is not None else None)
         return out
     at = blocks.long()
     x = dequantise_ref(cache.view(torch.uint8)[at].view(FP8), scale[at], out.dtype)
