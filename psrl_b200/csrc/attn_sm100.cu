@@ -86,6 +86,36 @@ __host__ __device__ constexpr uint64_t step_k(int k, int atom) { return (uint64_
 __host__ __device__ constexpr uint64_t step_mn(int k) { return (uint64_t)(k * 2048 >> 4); }
 constexpr uint64_t units(int bytes) { return (uint64_t)(bytes >> 4); }
 
+// Scores of the columns a row does not see become -inf: those past lim, and with a
+// window those before lo that are no sinks (>= sk; lim and lo are the row's, sk is
+// the tile's).  Most tiles cross one limit only, so that one comparison per column
+// does: the causal edge, the window's edge, or the tile that only holds sinks.
+template <bool WIN>
+__device__ __forceinline__ void mask_scores(uint32_t* v, int lim, int lo, int sk) {
+  constexpr uint32_t NINF = 0xff800000u;
+  const bool causal = __any_sync(0xffffffffu, lim < 127);
+  const bool window = WIN && __any_sync(0xffffffffu, lo > 0 && sk < 128);
+  if (!window) {
+    if (causal) {
+#pragma unroll
+      for (int i = 0; i < 128; ++i)
+        if (i > lim) v[i] = NINF;
+    }
+  } else if (!causal && sk <= 0) {
+#pragma unroll
+    for (int i = 0; i < 128; ++i)
+      if (i < lo) v[i] = NINF;
+  } else if (!causal && __all_sync(0xffffffffu, lo >= 128)) {
+#pragma unroll
+    for (int i = 0; i < 128; ++i)
+      if (i >= sk) v[i] = NINF;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 128; ++i)
+      if (i > lim || (i < lo && i >= sk)) v[i] = NINF;
+  }
+}
+
 // First failure of the launch: code, then (block x, y, z, warp, iteration) in err[1..5].
 __device__ __forceinline__ void set_err(int* err, int code, int it = -1) {
   if (err && atomicCAS(err, 0, code) == 0) {
@@ -297,7 +327,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       const int lim = row_pos + off - key0;  // last key column of the tile this row sees
       const int lo = lim - a.window + 1, sk = a.sinks - key0;  // WIN: columns from lo on, and those before sk
-      const bool masked_tile = __any_sync(0xffffffffu, lim < BKV - 1 || (WIN && lo > 0 && sk < BKV));
       // the whole S row (128 fp32 columns) comes out of TMEM in four loads
       // behind one wait and stays in registers for both passes
       uint32_t v[128];
@@ -306,11 +335,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       tmem_ld32(ts + 64, v + 64);
       tmem_ld32(ts + 96, v + 96);
       tmem_wait_ld();
-      if (masked_tile) {
-#pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i > lim || (WIN && i < lo && i >= sk)) v[i] = 0xff800000u;  // -inf: a key this row does not see
-      }
+      mask_scores<WIN>(v, lim, lo, sk);
       // pass 1: row maximum of the raw scores; the scale is positive, so it is
       // applied once, to the maximum
       float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -472,31 +497,39 @@ __global__ void fa_bwd_dot(const bf16* __restrict__ o, const bf16* __restrict__ 
                            const float* __restrict__ lse, float* __restrict__ lse2, float* __restrict__ dd,
                            const int* __restrict__ cu_end, bf16* __restrict__ dq,
                            int64_t dq_row, int dq_col, bf16* __restrict__ dkv, int64_t dkv_row, int dkv_cols) {
-  const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
+  // half a warp per (token, head)
+  const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
+  const int lane = threadIdx.x & 15;
   if (w >= T * nq) return;
   const int64_t t = w / nq;
   const int h = (int)(w - t * nq);
   if (cu_end && t >= *cu_end) {
     // a row behind the last sequence: its gradients are zeros (head 0's warp also
     // clears the key and value columns where they lie in the same tensor)
-    *reinterpret_cast<uint2*>(dq + t * dq_row + dq_col + (int64_t)h * D + lane * 4) = make_uint2(0, 0);
+    *reinterpret_cast<uint4*>(dq + t * dq_row + dq_col + (int64_t)h * D + lane * 8) = make_uint4(0, 0, 0, 0);
     if (h == 0)
-      for (int c = lane * 4; c < dkv_cols; c += 128)
-        *reinterpret_cast<uint2*>(dkv + t * dkv_row + c) = make_uint2(0, 0);
+      for (int c = lane * 8; c < dkv_cols; c += 128)
+        *reinterpret_cast<uint4*>(dkv + t * dkv_row + c) = make_uint4(0, 0, 0, 0);
     return;
   }
-  const bf16* po = o + w * D + lane * 4;
-  const bf16* pd = dout + w * D + lane * 4;
-  float s = 0.f;
+  // two sums of four products each, then over the lanes in halving distances
+  const unsigned mine = 0xffffu << (threadIdx.x & 16);  // the warp's other half may have left
+  float fo[8], fd[8], s4[2] = {0.f, 0.f};
+  unpack8(*reinterpret_cast<const bf16x8*>(o + w * D + lane * 8), fo);
+  unpack8(*reinterpret_cast<const bf16x8*>(dout + w * D + lane * 8), fd);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s += __bfloat162float(po[i]) * __bfloat162float(pd[i]);
+  for (int i = 0; i < 8; ++i) s4[i >> 2] += fo[i] * fd[i];
   if (o_lo) {
-    const bf16* pl = o_lo + w * D + lane * 4;
+    unpack8(*reinterpret_cast<const bf16x8*>(o_lo + w * D + lane * 8), fo);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s += __bfloat162float(pl[i]) * __bfloat162float(pd[i]);
+    for (int i = 0; i < 8; ++i) s4[i >> 2] += fo[i] * fd[i];
   }
-  s = warp_sum(s);
+#pragma unroll
+  for (int m = 8; m > 0; m >>= 1) {
+    s4[0] += __shfl_xor_sync(mine, s4[0], m, 16);
+    s4[1] += __shfl_xor_sync(mine, s4[1], m, 16);
+  }
+  const float s = s4[0] + s4[1];
   if (lane == 0) {
     dd[(int64_t)h * T + t] = s;
     lse2[(int64_t)h * T + t] = lse[(int64_t)h * T + t] * 1.4426950408889634f;
@@ -729,6 +762,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const int key = j * BKV + r;
     const int col0 = half * 32;
+    const int q_end = WIN && key >= a.sinks ? (int)min((int64_t)L - 1, (int64_t)key - off + a.window - 1) : L - 1;
     bool ok = true;
     for (int it = 0; it < iters; ++it) {
       const int i = i0 + it % per_head;
@@ -760,8 +794,9 @@ __global__ void __launch_bounds__(NT_BWD, 1)
         // are finite; rows past the sequence were loaded as zeros)
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
+          // the queries that see this key: from key - off up to q_end
           const int q = i * BQ2 + col0 + e;
-          if (!(q < L && key <= q + off && (!WIN || q + off - key < a.window || key < a.sinks))) {
+          if (!(q <= q_end && key <= q + off)) {
             vs[e] = 0xff800000u;
             if (WIN) vp[e] = 0;
           }
@@ -1009,6 +1044,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bqd);
     }
+    const int key_end = qin ? q + off : -1, key_lo = WIN ? q + off - a.window + 1 : 0;
     const float lse2 = qin ? a.lse[(int64_t)h * a.T + s0 + q] : 0.f;
     const float dd = qin ? a.dd[(int64_t)h * a.T + s0 + q] : 0.f;
     const int col0 = half * 32;
@@ -1037,8 +1073,9 @@ __global__ void __launch_bounds__(NT_BWD, 1)
         // masked scores become -inf, so P = 0 and dS = P (dP - D) = 0
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
+          // the keys that this query sees: up to key_end, from key_lo on or sinks
           const int key = key0 + col0 + e;
-          if (!(qin && key <= q + off && (!WIN || q + off - key < a.window || key < a.sinks))) {
+          if (key > key_end || (WIN && key < key_lo && key >= a.sinks)) {
             vs[e] = 0xff800000u;
             if (WIN) vp[e] = 0;
           }
@@ -1215,8 +1252,8 @@ static void bwd_launch(const at::Tensor& q, const at::Tensor& kv, const at::Tens
   auto dd = at::empty({nq, T}, q.options().dtype(at::kFloat)), lse2 = at::empty_like(dd);
   const bool same = dq.data_ptr() == dkv.data_ptr();  // one [q | k | v] gradient
   {
-    const int64_t warps = T * nq;
-    fa_bwd_dot<<<(unsigned)((warps * 32 + 255) / 256), 256, 0, stream()>>>(
+    const int64_t rows = T * nq;
+    fa_bwd_dot<<<(unsigned)((rows * 16 + 255) / 256), 256, 0, stream()>>>(
         reinterpret_cast<const bf16*>(o.data_ptr()),
         o_lo.has_value() ? reinterpret_cast<const bf16*>(o_lo->data_ptr()) : nullptr,
         reinterpret_cast<const bf16*>(dout.data_ptr()), T, (int)nq, lse.data_ptr<float>(), lse2.data_ptr<float>(),
