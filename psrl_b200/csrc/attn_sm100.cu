@@ -31,9 +31,10 @@
 // Sliding window (WIN): row p sees the keys with p + off - key < window, and the
 // first `sinks` keys.  The block's key tiles are then the sinks' tiles [0, ns)
 // and the window's, from w0 on; tile B skips the first of those where its window
-// starts a tile later.  Only tiles that cross a limit are masked, so a window
-// costs (window + 256 or so) / length of the causal time: measured forward, 32
-// heads, 16384 tokens: see the table of figures at the launcher.
+// starts a tile later.  Only tiles that cross a limit are masked.  Measured on a
+// B200, 16384 tokens, 32 q / 8 kv heads: full causal 1.84 ms forward, 8.1 ms
+// backward; window 4096 1.28 ms (754 TFLOP/s of the visible pairs; it sums the
+// rounded weights as well and writes o's rounding residue) and 4.1 ms (581).
 //
 // Work per block: tile A needs the key tiles up to its last row's limit,
 // tile B one more or two; only tiles that cross a row's limit are masked.  Blocks are launched

@@ -31,6 +31,12 @@
 //  * The exponents cost nothing per element: 2^ek scales a row of S^T, and
 //    P 2^ev is the second product's operand, with the running maximum taken over
 //    log2(p) + ev so that it stays within f16's range.
+//
+// Measured on a B200: 48 sequences up to 32768 tokens, 32 q / 8 kv heads, 336 us
+// (6.3 TB/s, 97% of copy bandwidth); 64 sequences up to 9216, 16 / 2 heads, 50 us
+// (4.1 TB/s: 28 tiles per CTA, so start, merge and join show); one of 517 tokens 10.8
+// us in a graph.  With the heads as rows (16 of them, half of them empty) and codes
+// converted by masks it was 555 us: 620 instructions per warp and tile against 400.
 #include "checks.cuh"
 #include "common.cuh"
 #include "driver_api.h"

@@ -17,7 +17,9 @@
 // before they are quantised (the numbers a bf16 cache would hold), max|x| as an
 // integer maximum over the eight lanes.  cos / sin stay in registers for the HV
 // heads a lane group handles.  Bound by HBM bytes: (nq + 2 nkv) * 2d in,
-// nq * 2d + 2 nkv (d + 1) out per token.
+// nq * 2d + 2 nkv (d + 1) out per token.  Measured on a B200: 10240 tokens at random
+// slots, 32 q / 8 kv heads, 50 us (4.7 TB/s); HV 1, 2 and 6 gave 54, 51 and 58.
+// read_kv_kernel: 3001 pages of 8 heads x 64 tokens 104 us (5.7 TB/s).
 #include <cuda_fp8.h>
 
 #include "common.cuh"
