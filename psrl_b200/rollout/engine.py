@@ -222,6 +222,8 @@ class RolloutEngine:
                                                    or self.block_size < 16 or self.block_size & (self.block_size - 1)):
             raise ValueError("an fp8 KV cache needs bf16 weights, head_dim 128 and a block size that is a power of two "
                              f">= 16, not {self.dtype}, {a.head_dim} and {self.block_size}")
+        if fp8 and self.device.type == "cuda" and self.max_model_len > 65536:
+            raise ValueError(f"an fp8 KV cache takes positions below 65536 (its rotary table), not {self.max_model_len}")
         self.kv_dtype = torch.float8_e4m3fn if fp8 else self.dtype
         vec_bytes = a.head_dim + 1 if fp8 else a.head_dim * torch.finfo(self.dtype).bits // 8
         per_block = 2 * a.num_layers * a.num_kv_heads * self.block_size * vec_bytes

@@ -235,3 +235,5 @@ def test_fp8_engine_refusals_gpu():
     w = EngineWeights.from_model(build_model(a, dev, torch.bfloat16, seed=1))
     with pytest.raises(ValueError, match="power of two"):
         RolloutEngine(a, w, max_model_len=256, block_size=24, num_blocks=16, kv_cache_dtype="fp8")
+    with pytest.raises(ValueError, match="65536"):
+        RolloutEngine(a, w, max_model_len=70000, block_size=64, num_blocks=2200, kv_cache_dtype="fp8")
