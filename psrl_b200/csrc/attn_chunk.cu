@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(threads_of(FP8), 1)
         if (!s_abort) set_err(a.err, 55);
         s_abort = 1;
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && elect_one()) {
       // --------------------------------------------------------- MMA issuer
       constexpr uint32_t idesc_qk = idesc_bf16_f32(BQ, BKV, false, false);
       constexpr uint32_t idesc_pv = idesc_bf16_f32(BQ, D, false, true);

@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc_qk = idesc_bf16_f32(BQ, BKV, false, false);
       constexpr uint32_t idesc_pv = idesc_bf16_f32(BQ, D, false, true);
       bool ok = mbar_wait(bq, 0);
@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(fb) : "memory");
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t id_ss = idesc_bf16_f32(BKV, BQ2, false, false);  // M = keys, N = 64 queries
       constexpr uint32_t id_ts = idesc_bf16_f32(BKV, D, false, true);     // M = keys, N = d, K = 64 queries
       const uint64_t dK = desc_sw128(smem_u32(smem), 16, 1024), dV = desc_sw128(smem_u32(smem) + KV_TILE, 16, 1024);
@@ -957,7 +957,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t id_s = idesc_bf16_f32(BQ, BK2, false, false);  // M = queries, N = 64 keys
       constexpr uint32_t id_dq = idesc_bf16_f32(BQ, D, false, true);    // M = queries, N = d, K = 64 keys
       const uint32_t kv0 = smem_u32(smem + OFF_DQ_KV);
