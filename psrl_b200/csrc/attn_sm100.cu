@@ -32,9 +32,9 @@
 // first `sinks` keys.  The block's key tiles are then the sinks' tiles [0, ns)
 // and the window's, from w0 on; tile B skips the first of those where its window
 // starts a tile later.  Only tiles that cross a limit are masked.  Measured on a
-// B200, 16384 tokens, 32 q / 8 kv heads: full causal 1.84 ms forward, 8.1 ms
-// backward; window 4096 1.28 ms (754 TFLOP/s of the visible pairs; it sums the
-// rounded weights as well and writes o's rounding residue) and 4.1 ms (581).
+// B200, 16384 tokens, 32 q / 8 kv heads: full causal 1.85 ms forward, 6.6 ms
+// backward; window 4096 1.27 ms (759 TFLOP/s of the visible pairs; it sums the
+// rounded weights as well and writes o's rounding residue) and 3.2 ms (755).
 //
 // Work per block: tile A needs the key tiles up to its last row's limit,
 // tile B one more or two; only tiles that cross a row's limit are masked.  Blocks are launched
@@ -81,8 +81,11 @@ struct FwdArgs {
 };
 
 // Descriptor steps in 16-byte units: the MMA thread adds one of these constants to
-// a base it keeps per operand.  (Composing a descriptor per MMA cost that single
-// thread about 100 cycles each, more than the product itself.)
+// a base it keeps per operand.  That thread's issue is what bounded the backward:
+// about 100 cycles per product with descriptors composed one by one in a branch on
+// the lane number; constants gave 8% (8.5 -> 8.1 ms, full causal, 16384 tokens), and
+// choosing the thread with elect.sync, whose operands then stay in uniform
+// registers, another 18% (6.6 ms).
 __host__ __device__ constexpr uint64_t step_k(int k, int atom) { return (uint64_t)(((k >> 2) * atom + (k & 3) * 32) >> 4); }
 __host__ __device__ constexpr uint64_t step_mn(int k) { return (uint64_t)(k * 2048 >> 4); }
 constexpr uint64_t units(int bytes) { return (uint64_t)(bytes >> 4); }
@@ -456,8 +459,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 //                dK += dS^T Q_i in TMEM (A operands from TMEM, B read MN-major).
 //   fa_bwd_dq    one CTA per (query head, sequence, 128-row tile i): Q_i and
 //                dO_i stay in tensor memory as A operands (a 128 x 64 product
-//                whose A comes from shared memory is bound by fetching it:
-//                measured 1970 cycles a step against 1024); for every key tile j <= i it
+//                whose A comes from shared memory fetches 6 KB for 32 cycles of
+//                products); for every key tile j <= i it
 //                recomputes S = Q_i K_j^T and dP = dO_i V_j^T, forms dS and
 //                accumulates dQ += dS K_j.
 // D = rowsum(dO * O) comes from fa_bwd_dot.  Softmax work uses eight warps,
@@ -682,7 +685,7 @@ __global__ void __launch_bounds__(NT_BWD, 1)
         tma_load_2d(sdo + ATOM64, &tm_do64, hq * D + 64, y, fb);
       }
       // lse and D of the 64 queries, asynchronously too: a producer that waited for
-      // plain loads here took 3200 cycles a step, the matrix products 1300
+      // plain loads here took 3200 cycles a step, and the MMA thread waited for it
 #pragma unroll
       for (int c = lane; c < 2 * BQ2; c += 32) {
         const int q = i * BQ2 + (c & (BQ2 - 1));
